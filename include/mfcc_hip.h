@@ -235,6 +235,127 @@ int mfcc_dct(const mfcc_plan* plan, const float* d_logmel, int64_t rows, float* 
 int mfcc_delta(const float* d_feats, const int64_t* d_frame_offsets, const int64_t* h_frame_offsets, int32_t n_utts,
                int32_t n_coef, int32_t width, int32_t order, float* d_out, void* stream);
 
+/* ---- operators over packed rows ------------------------------------------------------------ */
+/* What a sequence model does next with the (total_frames, channels) rows of a ragged batch: a short
+ * causal convolution, a selective state space scan and the norms around a block, each with its
+ * gradients and, for the first two, a form for single tokens.  No counterpart in the reference's
+ * feature path; they take the rows and frame offsets mfcc_execute works with.
+ *
+ *   - rows are row-major with unit stride along the channels; *_stride is the distance between rows
+ *     in elements (>= channels for outputs), so a column range of a wider matrix is a valid input;
+ *   - sequence s holds the rows d_offsets[s] .. d_offsets[s + 1] (ascending, n_seqs + 1 of them); a
+ *     NULL d_offsets with n_seqs = 1 is one sequence of all rows.  The offsets are read on the device
+ *     only, so a captured graph may be replayed with other offsets; values out of order or out of
+ *     range are never used as addresses.  Rows in no sequence are left as they are, or written as
+ *     zeros when zero_rest != 0; their gradients are zero;
+ *   - activations are MFCC_F32, MFCC_BF16 or MFCC_F16; learned tables, their gradients and the
+ *     scan's states are float32; all arithmetic is float32, rounded once into the output;
+ *   - sums run in a fixed order: the same call gives the same bits;
+ *   - everything is asynchronous on `stream`, allocates nothing and can be captured. */
+enum { MFCC_F32 = 0, MFCC_BF16 = 1, MFCC_F16 = 2 };
+enum { MFCC_ACT_NONE = 0, MFCC_ACT_SILU = 1 };
+
+/* Causal convolution of width 1 .. 8 along each sequence, channel by channel:
+ *   p[t, c] = bias[c] + sum_j weight[c, j] x[t - (width - 1) + j, c];  y = p, or p * sigmoid(p).
+ * State (n_seqs, width - 1, channels), of the element type: the rows before a sequence (d_initial,
+ * NULL: zeros) and its last rows (d_state, NULL: not wanted; must not alias d_initial). */
+typedef struct mfcc_conv_args {
+    int32_t struct_size;          /* sizeof(mfcc_conv_args) */
+    int32_t dtype, channels, width, activation, n_seqs, zero_rest;
+    int64_t rows;
+    const int64_t* d_offsets;
+    const void* d_x; int64_t x_stride;
+    const float* d_weight;        /* (channels, width) */
+    const float* d_bias;          /* (channels) or NULL */
+    const void* d_initial;
+    void* d_y; int64_t y_stride;  /* forward */
+    void* d_state;
+    const void* d_dy; int64_t dy_stride;   /* backward: gradients of y and, or NULL, of the state left behind */
+    const void* d_dstate;
+    void* d_dx; int64_t dx_stride;
+    float* d_dweight;
+    float* d_dbias;               /* NULL: not wanted */
+    void* d_dinitial;             /* NULL: not wanted */
+    void* d_workspace; size_t workspace_bytes;
+} mfcc_conv_args;
+int mfcc_causal_conv(const mfcc_conv_args* args, void* stream);
+size_t mfcc_causal_conv_backward_workspace(const mfcc_conv_args* args);
+int mfcc_causal_conv_backward(const mfcc_conv_args* args, void* stream);
+/* One token for each of `batch` entries: entry e continues the sequence whose state is row d_slots[e]
+ * (row e when d_slots is NULL) of d_state (n_slots, width - 1, channels); the state after the token goes
+ * to the same row of d_new_state, which may be d_state.  Entries that name one slot are successive tokens
+ * of it, in their order.  A slot outside [0, n_slots) is a padded entry: its row of y is zero. */
+int mfcc_causal_conv_step(int32_t dtype, int32_t batch, int32_t n_slots, int32_t channels, int32_t width,
+                          int32_t activation, const void* d_x, int64_t x_stride, const void* d_state, void* d_new_state,
+                          const float* d_weight, const float* d_bias, const int32_t* d_slots, void* d_y, int64_t y_stride,
+                          void* stream);
+
+/* Selective state space scan, 1 <= state <= 64, channels a multiple of groups; channel c reads the B and C
+ * rows of group c / (channels / groups):
+ *   d = softplus(delta + delta_bias) or delta + delta_bias
+ *   h[c, n] = exp(d A[c, n]) h[c, n] + d u[c] B[n];   y[c] = sum_n C[n] h[c, n] + D[c] u[c].
+ * d_initial / d_final (n_seqs, channels, state) float32: the state before and after each sequence. */
+typedef struct mfcc_scan_args {
+    int32_t struct_size;          /* sizeof(mfcc_scan_args) */
+    int32_t dtype, channels, state, groups, softplus, n_seqs, zero_rest;
+    int64_t rows;
+    const int64_t* d_offsets;
+    const void* d_u; int64_t u_stride;
+    const void* d_delta; int64_t delta_stride;
+    const float* d_A;             /* (channels, state) */
+    const void* d_B; int64_t B_stride;    /* (rows, groups, state): group and state contiguous */
+    const void* d_C; int64_t C_stride;
+    const float* d_D;             /* (channels) or NULL */
+    const float* d_delta_bias;    /* (channels) or NULL */
+    const float* d_initial;
+    void* d_y; int64_t y_stride;  /* forward */
+    float* d_final;               /* NULL: not wanted; must not alias d_initial */
+    const void* d_dy; int64_t dy_stride;  /* backward */
+    const float* d_dfinal;        /* gradient of d_final or NULL */
+    void* d_du; void* d_ddelta;   /* (rows, channels) contiguous */
+    float* d_dA;
+    void* d_dB; void* d_dC;       /* (rows, groups, state) contiguous */
+    float* d_dD; float* d_ddelta_bias; float* d_dinitial;   /* NULL: not wanted */
+    void* d_workspace; size_t workspace_bytes;
+} mfcc_scan_args;
+size_t mfcc_selective_scan_workspace(const mfcc_scan_args* args);
+int mfcc_selective_scan(const mfcc_scan_args* args, void* stream);
+size_t mfcc_selective_scan_backward_workspace(const mfcc_scan_args* args);
+int mfcc_selective_scan_backward(const mfcc_scan_args* args, void* stream);
+/* One token for each of args->rows entries; d_initial is the pool of states (n_slots, channels, state),
+ * d_final the pool they go to (may be d_initial), slots as in mfcc_causal_conv_step. */
+int mfcc_selective_scan_step(const mfcc_scan_args* args, int32_t n_slots, const int32_t* d_slots, void* stream);
+
+/* Norms before and after a block.  norm: MFCC_NORM_RMS v / sqrt(mean(v^2) + eps), MFCC_NORM_LAYER the same
+ * of v - mean(v).
+ *   add:   r = residual + scale * x;  y = norm(r) * weight + bias.  residual NULL: zero; scale a number
+ *          (scale_value) or, when d_scale is set, one per channel.  residual and r are of res_dtype.
+ *   gate:  y = norm(x * silu(z)) * weight + bias, or, with gate_first = 0, (norm(x) * weight + bias) * silu(z);
+ *          the norm runs over each of `groups` equal slices of the row. */
+enum { MFCC_NORM_RMS = 0, MFCC_NORM_LAYER = 1 };
+typedef struct mfcc_norm_args {
+    int32_t struct_size;          /* sizeof(mfcc_norm_args) */
+    int32_t dtype, res_dtype, channels, groups, norm, gate_first;
+    float eps, scale_value;
+    int64_t rows;
+    const float *d_weight, *d_bias, *d_scale;      /* each may be NULL */
+    const void* d_x; int64_t x_stride;
+    const void* d_z; int64_t z_stride;             /* gate */
+    const void* d_residual; int64_t residual_stride;
+    void* d_y; int64_t y_stride;                   /* forward */
+    void* d_r; int64_t r_stride;                   /* add: output of the forward, input of the backward pass */
+    const void* d_dy; int64_t dy_stride;           /* backward; add: d_dy or d_dr may be NULL (zero) */
+    const void* d_dr; int64_t dr_stride;
+    void* d_dx; void* d_dz; void* d_dresidual;     /* contiguous; add: NULL dresidual or dx: not wanted */
+    float *d_dweight, *d_dbias, *d_dscale;         /* NULL: not wanted; d_dscale needs d_x */
+    void* d_workspace; size_t workspace_bytes;
+} mfcc_norm_args;
+int mfcc_add_norm(const mfcc_norm_args* args, void* stream);
+int mfcc_gate_norm(const mfcc_norm_args* args, void* stream);
+size_t mfcc_norm_backward_workspace(const mfcc_norm_args* args);
+int mfcc_add_norm_backward(const mfcc_norm_args* args, void* stream);
+int mfcc_gate_norm_backward(const mfcc_norm_args* args, void* stream);
+
 /* ---- host helper for the 16-bit ingest ----------------------------------------------------- */
 /* h_dst[i] = h_src[i] * 32768 as int16.  Returns 1 if every sample lies on the int16 grid (the
  * product is an integer in [-32768, 32767]: what torchaudio yields for the 16-bit FLAC of

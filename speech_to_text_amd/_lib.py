@@ -53,6 +53,44 @@ class MfccConfigC(C.Structure):
     ]
 
 
+def _fields(text: str):
+    """ctypes fields from "type name, name; ..." lines in the order of the C struct."""
+    kinds = {"i32": C.c_int32, "i64": C.c_int64, "f32": C.c_float, "ptr": C.c_void_p, "size": C.c_size_t}
+    out = []
+    for group in text.split(";"):
+        kind, _, names = group.strip().partition(" ")
+        out += [(n.strip(), kinds[kind]) for n in names.split(",")]
+    return out
+
+
+class ConvArgsC(C.Structure):
+    """``struct mfcc_conv_args`` -- field order and types must match include/mfcc_hip.h."""
+
+    _fields_ = _fields("""i32 struct_size, dtype, channels, width, activation, n_seqs, zero_rest; i64 rows;
+        ptr d_offsets, d_x; i64 x_stride; ptr d_weight, d_bias, d_initial, d_y; i64 y_stride; ptr d_state, d_dy;
+        i64 dy_stride; ptr d_dstate, d_dx; i64 dx_stride; ptr d_dweight, d_dbias, d_dinitial, d_workspace;
+        size workspace_bytes""")
+
+
+class ScanArgsC(C.Structure):
+    """``struct mfcc_scan_args`` -- field order and types must match include/mfcc_hip.h."""
+
+    _fields_ = _fields("""i32 struct_size, dtype, channels, state, groups, softplus, n_seqs, zero_rest; i64 rows;
+        ptr d_offsets, d_u; i64 u_stride; ptr d_delta; i64 delta_stride; ptr d_A, d_B; i64 B_stride; ptr d_C;
+        i64 C_stride; ptr d_D, d_delta_bias, d_initial, d_y; i64 y_stride; ptr d_final, d_dy; i64 dy_stride;
+        ptr d_dfinal, d_du, d_ddelta, d_dA, d_dB, d_dC, d_dD, d_ddelta_bias, d_dinitial, d_workspace;
+        size workspace_bytes""")
+
+
+class NormArgsC(C.Structure):
+    """``struct mfcc_norm_args`` -- field order and types must match include/mfcc_hip.h."""
+
+    _fields_ = _fields("""i32 struct_size, dtype, res_dtype, channels, groups, norm, gate_first; f32 eps, scale_value;
+        i64 rows; ptr d_weight, d_bias, d_scale, d_x; i64 x_stride; ptr d_z; i64 z_stride; ptr d_residual;
+        i64 residual_stride; ptr d_y; i64 y_stride; ptr d_r; i64 r_stride; ptr d_dy; i64 dy_stride; ptr d_dr;
+        i64 dr_stride; ptr d_dx, d_dz, d_dresidual, d_dweight, d_dbias, d_dscale, d_workspace; size workspace_bytes""")
+
+
 class LibraryError(RuntimeError):
     """A call into libmfcc_hip failed; ``code`` is the MFCC_E_* value."""
 
@@ -120,6 +158,20 @@ SYMBOLS = {
     "mfcc_cmvn_accumulate": (C.c_int, [C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_void_p]),
     "mfcc_cmvn_apply": (C.c_int, [C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_double,
                                   C.c_void_p]),
+    "mfcc_causal_conv": (C.c_int, [C.POINTER(ConvArgsC), C.c_void_p]),
+    "mfcc_causal_conv_backward_workspace": (C.c_size_t, [C.POINTER(ConvArgsC)]),
+    "mfcc_causal_conv_backward": (C.c_int, [C.POINTER(ConvArgsC), C.c_void_p]),
+    "mfcc_causal_conv_step": (C.c_int, [C.c_int32] * 6 + [C.c_void_p, C.c_int64] + [C.c_void_p] * 6 + [C.c_int64, C.c_void_p]),
+    "mfcc_selective_scan_workspace": (C.c_size_t, [C.POINTER(ScanArgsC)]),
+    "mfcc_selective_scan": (C.c_int, [C.POINTER(ScanArgsC), C.c_void_p]),
+    "mfcc_selective_scan_backward_workspace": (C.c_size_t, [C.POINTER(ScanArgsC)]),
+    "mfcc_selective_scan_backward": (C.c_int, [C.POINTER(ScanArgsC), C.c_void_p]),
+    "mfcc_selective_scan_step": (C.c_int, [C.POINTER(ScanArgsC), C.c_int32, C.c_void_p, C.c_void_p]),
+    "mfcc_add_norm": (C.c_int, [C.POINTER(NormArgsC), C.c_void_p]),
+    "mfcc_gate_norm": (C.c_int, [C.POINTER(NormArgsC), C.c_void_p]),
+    "mfcc_norm_backward_workspace": (C.c_size_t, [C.POINTER(NormArgsC)]),
+    "mfcc_add_norm_backward": (C.c_int, [C.POINTER(NormArgsC), C.c_void_p]),
+    "mfcc_gate_norm_backward": (C.c_int, [C.POINTER(NormArgsC), C.c_void_p]),
 }
 
 _LIB = None

@@ -47,6 +47,18 @@ int fail(int code, const std::string& msg) {
     return code;
 }
 
+}  // namespace
+
+// The same convention for the other translation units (packed_*.hip).
+namespace mfcc_detail {
+int fail(int code, const char* msg) {
+    try { g_err = msg; } catch (...) {}
+    return code;
+}
+}  // namespace mfcc_detail
+
+namespace {
+
 #define HIP_TRY(expr)                                                                     \
     do {                                                                                  \
         hipError_t e_ = (expr);                                                           \

@@ -1,0 +1,190 @@
+// Shared by the operators over packed rows (packed_conv.hip, packed_scan.hip, packed_norm.hip):
+// element types, wide loads at any element alignment, the place of a row in its sequence, wavefront
+// sums, and the error convention of the C ABI.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <cstring>
+#include <new>
+#include <string>
+
+#include "../../include/mfcc_hip.h"
+
+namespace mfcc_detail {
+int fail(int code, const char* msg);     // sets the thread-local message behind mfcc_last_error(); never throws
+}
+
+#define PACKED_CATCH_ALL                                                              \
+    catch (const std::bad_alloc&) {                                                   \
+        return mfcc_detail::fail(MFCC_E_NOMEM, "out of host memory");                 \
+    } catch (...) {                                                                   \
+        return mfcc_detail::fail(MFCC_E_INVALID, "unexpected C++ exception");         \
+    }
+
+#define PACKED_LAUNCHED()                                                             \
+    do {                                                                              \
+        const hipError_t e_ = hipGetLastError();                                      \
+        if (e_ != hipSuccess) return mfcc_detail::fail(MFCC_E_HIP, hipGetErrorString(e_)); \
+    } while (0)
+
+namespace packed {
+
+constexpr int WAVE = 64;
+
+// ---- element types ---------------------------------------------------------------------------
+// Every operator computes in float32; the 16-bit types exist in memory only.  The conversions to
+// them round once, to nearest even (v_cvt_pk_bf16_f32 / v_cvt_f16_f32).
+struct F32 { using mem = float; };
+struct BF16 { using mem = __bf16; };
+struct F16 { using mem = _Float16; };
+
+template <typename M> __device__ __forceinline__ float widen(M v) { return (float)v; }
+template <typename M> __device__ __forceinline__ M narrow(float v) { return (M)v; }
+
+// VEC elements from an address that is only aligned to its element: global memory takes wide accesses
+// at any such address on gfx950, so a row of any width and stride uses the same 16-byte loads.
+// n < VEC (the ragged end of a row) goes element by element.
+template <typename M, int VEC>
+__device__ __forceinline__ void load_vec(float (&v)[VEC], const M* __restrict__ p, int n) {
+    if (n >= VEC) {
+        M raw[VEC];
+        __builtin_memcpy(raw, p, sizeof(raw));
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[i] = widen(raw[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[i] = i < n ? widen(p[i]) : 0.0f;
+    }
+}
+
+template <typename M, int VEC>
+__device__ __forceinline__ void store_vec(M* __restrict__ p, const float (&v)[VEC], int n) {
+    if (n >= VEC) {
+        M raw[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) raw[i] = narrow<M>(v[i]);
+        __builtin_memcpy(p, raw, sizeof(raw));
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+            if (i < n) p[i] = narrow<M>(v[i]);
+    }
+}
+
+// ---- functions ---------------------------------------------------------------------------------
+constexpr float LOG2E = 1.44269504088896340736f;
+constexpr float LN2 = 0.69314718055994530942f;
+
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float log2_hw(float x) { return __builtin_amdgcn_logf(x); }
+__device__ __forceinline__ float rcp_hw(float x) { return __builtin_amdgcn_rcpf(x); }
+
+// exp(x): the product with log2(e) is carried in two floats, so that its rounding does not grow with |x|.
+__device__ __forceinline__ float exp_f(float x) {
+    const float p = x * LOG2E;
+    const float lo = fmaf(x, LOG2E, -p) + x * 1.92596299e-8f;    // the rest of x * log2(e); NaN for infinite x
+    const float e = exp2_hw(p);
+    // outside the finite, normal range the correction is meaningless (and inf * 0 or inf - inf appears in it)
+    return fabsf(p) < 126.0f ? fmaf(e * LN2, lo, e) : e;
+}
+
+__device__ __forceinline__ float sigmoid_f(float x) { return rcp_hw(1.0f + exp_f(-x)); }
+
+// log(1 + exp(x)) = max(x, 0) + log(1 + e), e = exp(-|x|) in (0, 1].  w = 1 + e loses the low bits of a
+// small e; what it lost, e - (w - 1), is exact and is added back (to first order: the error of that is
+// below 2^-24 e).
+__device__ __forceinline__ float softplus_f(float x) {
+    const float e = exp_f(-fabsf(x));
+    const float w = 1.0f + e;
+    return fmaxf(x, 0.0f) + fmaf(log2_hw(w), LN2, e - (w - 1.0f));
+}
+
+// ---- where a row lies ----------------------------------------------------------------------------
+// Sequence s holds the rows off[s] .. off[s + 1].  The offsets are device data that no host code has
+// seen, so nothing read from them is trusted as an index: a row that is inside the sequence found for it
+// satisfies 0 <= start <= row < end, and rows are never addressed outside [0, rows).
+struct Place {
+    int s;               // sequence, in [0, n_seqs)
+    int64_t start, end;  // its rows (start <= row < end) when inside, clipped to [0, rows]
+    int64_t until;       // first row at which this answer may change (> row)
+    bool inside;
+};
+
+__device__ __forceinline__ Place find_row(const int64_t* __restrict__ off, int n_seqs, int64_t rows, int64_t row) {
+    Place p;
+    if (!off) {          // one sequence of all rows
+        p.s = 0; p.start = 0; p.end = rows; p.until = rows; p.inside = row < rows;
+        return p;
+    }
+    int lo = 0, hi = n_seqs;                    // the last s with off[s] <= row, or 0
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (off[mid] <= row) lo = mid; else hi = mid;
+    }
+    p.s = lo;
+    p.start = off[lo];
+    p.end = min(off[lo + 1], rows);
+    p.inside = p.start >= 0 && p.start <= row && row < p.end;
+    if (p.inside) p.until = p.end;
+    else if (row < p.start) p.until = min(p.start, rows);          // before the first sequence
+    else if (lo == n_seqs - 1) p.until = rows;                     // behind the last one
+    else p.until = row + 1;                                        // offsets that do not ascend
+    return p;
+}
+
+// ---- wavefront helpers ----------------------------------------------------------------------------
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+
+// lanes 0..31: x summed with its upper half; lanes 32..63: y summed with its lower half
+__device__ __forceinline__ float halve32(float x, float y) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// even rows of 16 lanes: x summed over the pair of rows; odd rows: y
+__device__ __forceinline__ float halve16(float x, float y) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Sum over the 64 lanes, in every lane.
+__device__ __forceinline__ float wave_sum(float v) {
+    v += dpp<0xB1>(v);          // quad_perm [1, 0, 3, 2]
+    v += dpp<0x4E>(v);          // quad_perm [2, 3, 0, 1]
+    v += dpp<0x141>(v);         // row_half_mirror
+    v += dpp<0x140>(v);         // row_mirror
+    v = halve16(v, v);
+    return halve32(v, v);
+}
+
+// Whether another entry of a batch names the slot of entry e0, before or after it.  Every wavefront looks
+// through the whole list by itself, 64 entries at a time.
+struct SlotUse { bool before, after; };
+__device__ __forceinline__ SlotUse slot_use(const int32_t* __restrict__ slots, int batch, int e0) {
+    const int slot = slots[e0];
+    bool before = false, after = false;
+    for (int e = threadIdx.x & 63; e < batch; e += WAVE) {
+        const bool same = slots[e] == slot;
+        before |= same && e < e0;
+        after |= same && e > e0;
+    }
+    return {__ballot(before) != 0, __ballot(after) != 0};
+}
+
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+template <typename Fn>
+int by_type(int dtype, Fn&& fn) {
+    switch (dtype) {
+        case MFCC_F32: return fn(F32{});
+        case MFCC_BF16: return fn(BF16{});
+        case MFCC_F16: return fn(F16{});
+    }
+    return mfcc_detail::fail(MFCC_E_INVALID, "unknown element type");
+}
+
+}  // namespace packed
