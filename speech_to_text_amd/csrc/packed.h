@@ -95,8 +95,9 @@ __device__ __forceinline__ float sigmoid_f(float x) { return rcp_hw(1.0f + exp_f
 // log(1 + exp(x)) = max(x, 0) + log(1 + e), e = exp(-|x|) in (0, 1].  w = 1 + e loses the low bits of a
 // small e; what it lost, e - (w - 1), is exact and is added back (to first order: the error of that is
 // below 2^-24 e).
+template <bool EXACT = true>
 __device__ __forceinline__ float softplus_f(float x) {
-    const float e = exp_f(-fabsf(x));
+    const float e = EXACT ? exp_f(-fabsf(x)) : exp2_hw(-fabsf(x) * LOG2E);
     const float w = 1.0f + e;
     return fmaxf(x, 0.0f) + fmaf(log2_hw(w), LN2, e - (w - 1.0f));
 }
@@ -132,6 +133,36 @@ __device__ __forceinline__ Place find_row(const int64_t* __restrict__ off, int n
     else if (lo == n_seqs - 1) p.until = rows;                     // behind the last one
     else p.until = row + 1;                                        // offsets that do not ascend
     return p;
+}
+
+// A value that is the same in all lanes, in a scalar register -- and, through the empty asm, known as such to
+// the compiler, which otherwise keeps loop counters that come out of a search in vector registers and
+// computes addresses and branches from them lane by lane.
+__device__ __forceinline__ int uniform(int v) {
+    v = __builtin_amdgcn_readfirstlane(v);
+    asm("" : "+s"(v));
+    return v;
+}
+
+// The same for a whole wavefront, in scalar registers and relative to row r0 of a piece of `len` rows: which
+// rows from t on lie in one sequence (or in none), and what happens at their ends.
+struct Stretch {
+    int s;               // sequence
+    int until;           // first row (<= len) at which the answer may change
+    int inside, first, last;    // in a sequence; row t is its first row; row until - 1 is its last one
+};
+
+__device__ __forceinline__ Stretch find_stretch(const int64_t* __restrict__ off, int n_seqs, int64_t rows, int64_t r0, int t,
+                                                int len) {
+    const Place p = find_row(off, n_seqs, rows, r0 + t);
+    Stretch w;
+    w.s = uniform(p.s);
+    w.until = uniform((int)min(p.until - r0, (int64_t)len));
+    const int flags = uniform((p.inside ? 1 : 0) | (p.start == r0 + t ? 2 : 0) | (p.end - r0 <= len ? 4 : 0));
+    w.inside = flags & 1;
+    w.first = flags & 2;
+    w.last = (flags & 5) == 5 ? 1 : 0;
+    return w;
 }
 
 // ---- wavefront helpers ----------------------------------------------------------------------------

@@ -19,6 +19,10 @@ namespace packed {
 constexpr float SCAN_LOG2E = LOG2E;
 constexpr int SCAN_TILE = 32;       // rows of B and C staged in LDS at a time (forward kernels)
 
+// Holds the LDS reads of the next row back until half of this row's states are done: hoisted by the compiler,
+// the B and C of four rows take the registers of two wavefronts.
+__device__ __forceinline__ void after(int& offset, float& state) { asm volatile("" : "+v"(offset), "+v"(state)); }
+
 struct Scan {
     const void *u, *delta, *B, *C, *dy;
     int64_t u_stride, delta_stride, B_stride, C_stride, dy_stride, y_stride;
@@ -33,11 +37,38 @@ struct Scan {
     int n_seqs, channels, state, groups, per, chunk, n_chunks, blocks_per_group, softplus, zero_rest;
 };
 
+// d of a row.  In the 16-bit types delta itself is rounded to 2^-9 and less, so softplus takes its exponential
+// without the second float of the exponent's product (|delta| 2^-24 more).
 template <typename M>
-__device__ __forceinline__ float step_of(const Scan& a, M raw, float bias) {
+__device__ __forceinline__ float step_of(int softplus, M raw, float bias) {
     const float v = widen(raw) + bias;
-    return a.softplus ? softplus_f(v) : v;
+    return softplus ? softplus_f<sizeof(M) == 4>(v) : v;
 }
+
+// The next rows of a wavefront's channels, loaded while the ones before them are worked on.  The row is in
+// scalar registers, the lane adds its channel.
+constexpr int AHEAD = 4;
+template <typename M, bool BACK>
+struct Ahead {
+    M u[AHEAD], delta[AHEAD], dy[BACK ? AHEAD : 1];
+    // rows t .. t + 3 of the chunk at r0, its last one instead of those behind it
+    __device__ __forceinline__ void load(const Scan& a, int64_t r0, int t, int len, unsigned c) {
+        const M* pu = static_cast<const M*>(a.u) + (r0 + t) * a.u_stride;
+        const M* pd = static_cast<const M*>(a.delta) + (r0 + t) * a.delta_stride;
+        const M* py = BACK ? static_cast<const M*>(a.dy) + (r0 + t) * a.dy_stride : nullptr;
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            u[j] = pu[c];
+            delta[j] = pd[c];
+            if (BACK) dy[j] = py[c];
+            if (t + j + 1 < len) {
+                pu += a.u_stride;
+                pd += a.delta_stride;
+                if (BACK) py += a.dy_stride;
+            }
+        }
+    }
+};
 
 // Channels of one workgroup of the kernels with a lane per channel: whole wavefronts, spread evenly over as
 // few workgroups of at most four wavefronts as a group of channels needs.
@@ -47,8 +78,8 @@ inline int scan_block(int per) {
 }
 
 // One row of B or C in LDS, read by all lanes at once.
-template <int NP>
-__device__ __forceinline__ void row_of(float (&v)[NP], const float* p) {
+template <int NP, int SIZE>
+__device__ __forceinline__ void row_of(float (&v)[SIZE], const float* p) {
 #pragma unroll
     for (int n = 0; n < NP; n += 4) {
         const float4 q = *reinterpret_cast<const float4*>(p + n);
@@ -63,6 +94,33 @@ __device__ __forceinline__ void stage_rows(float* lds, const M* __restrict__ src
         const int n = i % NP;
         lds[i] = n < state ? widen(src[(row + i / NP) * stride + n]) : 0.0f;
     }
+}
+
+// A channel's states in an (sequence, channel, n) array; zeros without the array.  Rarely run inside the loop
+// over rows: the opaque offset and count keep the compiler from holding its sixteen addresses and lane masks in
+// registers throughout.
+template <int NP>
+__device__ __forceinline__ void load_state(float (&v)[NP], const float* from, const Scan& a, int s, int c) {
+#pragma unroll
+    for (int n = 0; n < NP; ++n) v[n] = 0.0f;
+    if (!from) return;
+    int64_t at = ((int64_t)s * a.channels + c) * a.state;
+    int count = a.state;
+    asm volatile("" : "+v"(at), "+s"(count));
+#pragma unroll
+    for (int n = 0; n < NP; ++n) {
+        const float x = from[at + min(n, count - 1)];
+        v[n] = n < count ? x : 0.0f;
+    }
+}
+template <int NP>
+__device__ __forceinline__ void store_state(float* to, const float (&v)[NP], const Scan& a, int s, int c) {
+    int64_t at = ((int64_t)s * a.channels + c) * a.state;
+    int count = a.state;
+    asm volatile("" : "+v"(at), "+s"(count));
+#pragma unroll
+    for (int n = 0; n < NP; ++n)
+        if (n < count) to[at + n] = v[n];
 }
 
 template <int NP>
@@ -82,10 +140,8 @@ __global__ __launch_bounds__(256) void k_scan_sum(const Scan a) {
     const int in_group = (cb % a.blocks_per_group) * blockDim.x + threadIdx.x;
     const bool live = in_group < a.per;
     const int c = g * a.per + (live ? in_group : 0);
-    const int64_t r0 = (int64_t)k * a.chunk, r1 = min(r0 + a.chunk, a.rows);
-    const M* u = static_cast<const M*>(a.u) + c;
-    const M* delta = static_cast<const M*>(a.delta) + c;
-    const M* dy = static_cast<const M*>(a.dy) + c;
+    const int64_t r0 = (int64_t)k * a.chunk;
+    const int len = (int)min((int64_t)a.chunk, a.rows - r0);
     const M* B = static_cast<const M*>(a.B) + (int64_t)g * a.state;
     const M* C = static_cast<const M*>(a.C) + (int64_t)g * a.state;
     const float bias = a.bias ? a.bias[c] : 0.0f;
@@ -95,49 +151,79 @@ __global__ __launch_bounds__(256) void k_scan_sum(const Scan a) {
 #pragma unroll
     for (int n = 0; n < NP; ++n) { h[n] = 0.0f; P[n] = 1.0f; R[n] = 0.0f; }
     float sum = 0.0f;
-    bool reset = false;            // a sequence start was passed: the reverse part is complete
+    int reset = 0;                 // a sequence start was passed: the reverse part is complete
 
-    Place q = find_row(a.off, a.n_seqs, a.rows, r0);
-    for (int64_t t0 = r0; t0 < r1; t0 += SCAN_TILE) {
-        const int64_t t1 = min(t0 + SCAN_TILE, r1);
+    Ahead<M, BACK> next;
+    next.load(a, r0, 0, len, c);
+    Stretch q = find_stretch(a.off, a.n_seqs, a.rows, r0, 0, len);
+    for (int t0 = 0; t0 < len; t0 += SCAN_TILE) {
+        const int t1 = min(t0 + SCAN_TILE, len);
         __syncthreads();
-        stage_rows<M, NP>(sB, B, a.B_stride, t0, (int)(t1 - t0), a.state);
-        if (BACK) stage_rows<M, NP>(sC, C, a.C_stride, t0, (int)(t1 - t0), a.state);
+        stage_rows<M, NP>(sB, B, a.B_stride, r0 + t0, t1 - t0, a.state);
+        if (BACK) stage_rows<M, NP>(sC, C, a.C_stride, r0 + t0, t1 - t0, a.state);
         __syncthreads();
-        for (int64_t r = t0; r < t1;) {
-            if (r >= q.until) q = find_row(a.off, a.n_seqs, a.rows, r);
-            const int64_t r2 = min(t1, q.until);
-            if (!q.inside || r == q.start) {
-                reset = true;
+        for (int t = t0; t < t1;) {
+            if (t >= q.until) q = find_stretch(a.off, a.n_seqs, a.rows, r0, t, len);
+            const int t2 = uniform(min(t1, q.until));
+            if (!q.inside || q.first) {
+                reset = uniform(1);
                 sum = 0.0f;
-#pragma unroll
-                for (int n = 0; n < NP; ++n)
-                    h[n] = q.inside && a.initial && n < a.state ? a.initial[((int64_t)q.s * a.channels + c) * a.state + n] : 0.0f;
+                load_state<NP>(h, q.inside ? a.initial : nullptr, a, q.s, c);
+                q.first = false;
             }
-            if (!q.inside) { r = r2; continue; }
-            for (; r < r2; ++r) {
-                const float d = step_of(a, delta[r * a.delta_stride], bias);
-                const float du = d * widen(u[r * a.u_stride]);
-                float b[NP], cc[NP];
-                row_of<NP>(b, sB + (r - t0) * NP);
-                if (BACK && !reset) {
-                    row_of<NP>(cc, sC + (r - t0) * NP);
-                    const float dv = widen(dy[r * a.dy_stride]);
-                    const bool last = a.dfinal && r + 1 == q.end;
+            if (!q.inside) {
+                t = t2;
+                if (t < len) next.load(a, r0, t, len, c);
+                continue;
+            }
+            // rows t .. t2 in groups of four; OPEN: the reverse part still runs
+            auto advance = [&](auto open) {
+                constexpr bool OPEN = decltype(open)::value;
+                while (t < t2) {
+                    const int from = t, count = uniform(min(AHEAD, t2 - t));
+                    const Ahead<M, BACK> now = next;
+                    t = uniform(t + count);
+                    if (t < len) next.load(a, r0, t, len, c);
+                    float d[AHEAD], du[AHEAD], dv[AHEAD];
 #pragma unroll
-                    for (int n = 0; n < NP; ++n) {
-                        const float e = exp2_hw(d * A2[n]);
-                        float v = cc[n] * dv;
-                        if (last && n < a.state) v += a.dfinal[((int64_t)q.s * a.channels + c) * a.state + n];
-                        P[n] *= e;
-                        R[n] = fmaf(P[n], v, R[n]);
-                        h[n] = fmaf(e, h[n], du * b[n]);
+                    for (int j = 0; j < AHEAD; ++j) {
+                        d[j] = step_of(a.softplus, now.delta[j], bias);
+                        du[j] = d[j] * widen(now.u[j]);
+                        dv[j] = OPEN ? widen(now.dy[j]) : 0.0f;
                     }
-                } else {
+                    if (count < AHEAD) {                   // rows behind the last: a step of zero changes nothing
 #pragma unroll
-                    for (int n = 0; n < NP; ++n) h[n] = fmaf(exp2_hw(d * A2[n]), h[n], du * b[n]);
+                        for (int j = 1; j < AHEAD; ++j)
+                            if (j >= count) d[j] = du[j] = dv[j] = 0.0f;
+                    }
+                    int at = (from - t0) * NP;
+#pragma unroll
+                    for (int j = 0; j < AHEAD; ++j) {
+                        float b[NP], cc[OPEN ? NP : 4];
+                        row_of<NP>(b, sB + at);
+                        if (OPEN) row_of<NP>(cc, sC + at);
+                        at += j + 1 < count ? NP : 0;
+#pragma unroll
+                        for (int n = 0; n < NP; ++n) {
+                            const float e = exp2_hw(d[j] * A2[n]);
+                            if (OPEN) {
+                                P[n] *= e;
+                                R[n] = fmaf(P[n], cc[n] * dv[j], R[n]);
+                            }
+                            h[n] = fmaf(e, h[n], du[j] * b[n]);
+                        }
+                        after(at, h[NP / 2]);
+                    }
+                    sum += (d[0] + d[1]) + (d[2] + d[3]);
                 }
-                sum += d;
+            };
+            if (BACK && !reset) advance(std::integral_constant<bool, BACK>{});
+            else advance(std::false_type{});
+            if (BACK && a.dfinal && !reset && q.last && t == q.until) {   // the gradient of the state left behind enters here
+                float g_end[NP];
+                load_state<NP>(g_end, a.dfinal, a, q.s, c);
+#pragma unroll
+                for (int n = 0; n < NP; ++n) R[n] = fmaf(P[n], g_end[n], R[n]);
             }
         }
     }
@@ -155,6 +241,7 @@ __global__ __launch_bounds__(256) void k_scan_sum(const Scan a) {
 
 // Pass 2, in place: hst[k] (and, from the right, gst[k]) becomes the state that enters chunk k.  64 columns
 // by 16 segments of the chunks: each segment's own composition, then the ones before it, then the segment.
+// Eight chunks are loaded at a time: one after the other they are a chain of memory latencies.
 template <typename T>
 __global__ __launch_bounds__(1024) void k_scan_carry(const Scan a) {
     __shared__ float sD[16][64], sH[16][64];
@@ -168,29 +255,44 @@ __global__ __launch_bounds__(1024) void k_scan_carry(const Scan a) {
     const float A2 = a.A[(int64_t)c * a.state + n] * SCAN_LOG2E;
     const int len = (a.n_chunks + 15) / 16;
     const int k0 = min(seg * len, a.n_chunks), k1 = min(k0 + len, a.n_chunks);
-    float D = 1.0f, H = 0.0f;
-    if (live)
-        for (int i = k0; i < k1; ++i) {
-            const int k = right ? a.n_chunks - 1 - i : i;
-            const float v = st[k * m + e];
-            const bool cut = a.reset[k] != 0;
-            const float dec = exp2_hw(A2 * a.dsum[(int64_t)k * a.channels + c]);
-            H = cut ? v : fmaf(dec, H, v);
-            D = cut ? 0.0f : D * dec;
+    constexpr int BATCH = 8;
+    float v[BATCH], dec[BATCH];
+    int cut[BATCH];
+    auto fetch = [&](int i0) {
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) {
+            const int i = min(i0 + j, k1 - 1), k = right ? a.n_chunks - 1 - i : i;
+            v[j] = live ? st[k * m + e] : 0.0f;
+            dec[j] = a.dsum[(int64_t)k * a.channels + c];
+            cut[j] = a.reset[k];
         }
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) dec[j] = exp2_hw(A2 * dec[j]);
+    };
+    float D = 1.0f, H = 0.0f;
+    for (int i0 = k0; i0 < k1; i0 += BATCH) {
+        fetch(i0);
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j)
+            if (i0 + j < k1) {
+                H = cut[j] ? v[j] : fmaf(dec[j], H, v[j]);
+                D = cut[j] ? 0.0f : D * dec[j];
+            }
+    }
     sD[seg][lane] = D; sH[seg][lane] = H;
     __syncthreads();
-    if (!live) return;
     float carry = 0.0f;
     // D == 0 also where a chunk of the segment is cut: nothing passes, whatever the carry is
     for (int s = 0; s < seg; ++s) carry = sD[s][lane] == 0.0f ? sH[s][lane] : fmaf(sD[s][lane], carry, sH[s][lane]);
-    for (int i = k0; i < k1; ++i) {
-        const int k = right ? a.n_chunks - 1 - i : i;
-        const float v = st[k * m + e];
-        const bool cut = a.reset[k] != 0;
-        const float dec = exp2_hw(A2 * a.dsum[(int64_t)k * a.channels + c]);
-        st[k * m + e] = carry;
-        carry = cut ? v : fmaf(dec, carry, v);
+    for (int i0 = k0; i0 < k1; i0 += BATCH) {
+        if (len > BATCH) fetch(i0);                    // a shorter segment is still in registers
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j)
+            if (i0 + j < k1) {
+                const int k = right ? a.n_chunks - 1 - (i0 + j) : i0 + j;
+                if (live) st[k * m + e] = carry;
+                carry = cut[j] ? v[j] : fmaf(dec[j], carry, v[j]);
+            }
     }
 }
 
@@ -205,10 +307,9 @@ __global__ __launch_bounds__(256) void k_scan_fwd(const Scan a) {
     const int in_group = (cb % a.blocks_per_group) * blockDim.x + threadIdx.x;
     const bool live = in_group < a.per;
     const int c = g * a.per + (live ? in_group : 0);
-    const int64_t r0 = (int64_t)k * a.chunk, r1 = min(r0 + a.chunk, a.rows);
-    const M* u = static_cast<const M*>(a.u) + c;
-    const M* delta = static_cast<const M*>(a.delta) + c;
-    M* y = static_cast<M*>(a.y) + c;
+    const int64_t r0 = (int64_t)k * a.chunk;
+    const int len = (int)min((int64_t)a.chunk, a.rows - r0);
+    M* y = static_cast<M*>(a.y);
     const M* B = static_cast<const M*>(a.B) + (int64_t)g * a.state;
     const M* C = static_cast<const M*>(a.C) + (int64_t)g * a.state;
     const float bias = a.bias ? a.bias[c] : 0.0f;
@@ -220,48 +321,73 @@ __global__ __launch_bounds__(256) void k_scan_fwd(const Scan a) {
     for (int n = 0; n < NP; ++n)
         h[n] = a.n_chunks > 1 && n < a.state ? a.hst[((int64_t)k * a.state + n) * a.channels + c] : 0.0f;
 
-    Place q = find_row(a.off, a.n_seqs, a.rows, r0);
-    for (int64_t t0 = r0; t0 < r1; t0 += SCAN_TILE) {
-        const int64_t t1 = min(t0 + SCAN_TILE, r1);
+    Ahead<M, false> next;
+    next.load(a, r0, 0, len, c);
+    Stretch q = find_stretch(a.off, a.n_seqs, a.rows, r0, 0, len);
+    for (int t0 = 0; t0 < len; t0 += SCAN_TILE) {
+        const int t1 = min(t0 + SCAN_TILE, len);
         __syncthreads();
-        stage_rows<M, NP>(sB, B, a.B_stride, t0, (int)(t1 - t0), a.state);
-        stage_rows<M, NP>(sC, C, a.C_stride, t0, (int)(t1 - t0), a.state);
+        stage_rows<M, NP>(sB, B, a.B_stride, r0 + t0, t1 - t0, a.state);
+        stage_rows<M, NP>(sC, C, a.C_stride, r0 + t0, t1 - t0, a.state);
         __syncthreads();
-        for (int64_t r = t0; r < t1;) {
-            if (r >= q.until) q = find_row(a.off, a.n_seqs, a.rows, r);
-            const int64_t r2 = min(t1, q.until);
+        for (int t = t0; t < t1;) {
+            if (t >= q.until) q = find_stretch(a.off, a.n_seqs, a.rows, r0, t, len);
+            const int t2 = uniform(min(t1, q.until));
             if (!q.inside) {
                 if (a.zero_rest && live)
-                    for (; r < r2; ++r) y[r * a.y_stride] = narrow<M>(0.0f);
-                r = r2;
+                    for (int i = t; i < t2; ++i) (y + (r0 + i) * a.y_stride)[(unsigned)c] = narrow<M>(0.0f);
+                t = t2;
+                if (t < len) next.load(a, r0, t, len, c);
                 continue;
             }
-            if (r == q.start) {
-#pragma unroll
-                for (int n = 0; n < NP; ++n)
-                    h[n] = a.initial && n < a.state ? a.initial[((int64_t)q.s * a.channels + c) * a.state + n] : 0.0f;
+            if (q.first) {
+                load_state<NP>(h, a.initial, a, q.s, c);
+                q.first = false;
             }
-            for (; r < r2; ++r) {
-                const float uv = widen(u[r * a.u_stride]);
-                const float d = step_of(a, delta[r * a.delta_stride], bias);
-                const float du = d * uv;
-                float b[NP], cc[NP];
-                row_of<NP>(b, sB + (r - t0) * NP);
-                row_of<NP>(cc, sC + (r - t0) * NP);
-                float acc = skip * uv;
-                if (!a.D) acc = 0.0f;
+            while (t < t2) {
+                const int from = t, count = uniform(min(AHEAD, t2 - t));
+                const Ahead<M, false> now = next;
+                t = uniform(t + count);
+                if (t < len) next.load(a, r0, t, len, c);
+                float d[AHEAD], du[AHEAD], out[AHEAD];
 #pragma unroll
-                for (int n = 0; n < NP; ++n) {
-                    h[n] = fmaf(exp2_hw(d * A2[n]), h[n], du * b[n]);
-                    acc = fmaf(cc[n], h[n], acc);
+                for (int j = 0; j < AHEAD; ++j) {
+                    const float uv = widen(now.u[j]);
+                    d[j] = step_of(a.softplus, now.delta[j], bias);
+                    du[j] = d[j] * uv;
+                    out[j] = skip * uv;
                 }
-                if (live) y[r * a.y_stride] = narrow<M>(acc);
-            }
-            if (a.final && r == q.end && live) {
+                if (count < AHEAD) {                       // rows behind the last: a step of zero changes nothing
 #pragma unroll
-                for (int n = 0; n < NP; ++n)
-                    if (n < a.state) a.final[((int64_t)q.s * a.channels + c) * a.state + n] = h[n];
+                    for (int j = 1; j < AHEAD; ++j)
+                        if (j >= count) d[j] = du[j] = 0.0f;
+                }
+                if (!a.D) {                                // no term at all, also where u is infinite
+#pragma unroll
+                    for (int j = 0; j < AHEAD; ++j) out[j] = 0.0f;
+                }
+                int at = (from - t0) * NP;
+#pragma unroll
+                for (int j = 0; j < AHEAD; ++j) {
+                    float b[NP], cc[NP];
+                    row_of<NP>(b, sB + at);
+                    row_of<NP>(cc, sC + at);
+                    at += j + 1 < count ? NP : 0;
+#pragma unroll
+                    for (int n = 0; n < NP; ++n) {
+                        h[n] = fmaf(exp2_hw(d[j] * A2[n]), h[n], du[j] * b[n]);
+                        out[j] = fmaf(cc[n], h[n], out[j]);
+                    }
+                    asm volatile("" : "+v"(out[j]));       // the sum is made here, not at the store (registers)
+                    after(at, h[NP / 2]);
+                }
+                if (live) {
+#pragma unroll
+                    for (int j = 0; j < AHEAD; ++j)
+                        if (j < count) (y + (r0 + from + j) * a.y_stride)[(unsigned)c] = narrow<M>(out[j]);
+                }
             }
+            if (a.final && q.last && t == q.until && live) store_state<NP>(a.final, h, a, q.s, c);
         }
     }
 }
@@ -280,13 +406,15 @@ __global__ __launch_bounds__(256) void k_scan_empty(const int64_t* __restrict__ 
 
 // ---- gradients ---------------------------------------------------------------------------------------
 // A lane holds four of a channel's states (LPC = NP / 4 lanes per channel), a workgroup of four wavefronts
-// 4 * 64 / LPC channels of one group and one chunk of rows.  The chunk's d, u, dy, B and C lie in LDS.  The
-// chunk is swept once forward, keeping the state at every eighth row, and then eight rows at a time from
-// its end: forward again with all eight states and decays in registers, and back over them.
+// 4 * 64 / LPC channels of one group and one chunk of rows.  The chunk's d, u and dy lie in LDS by channel (eight
+// rows of a channel are one or two 16-byte reads; the padding spreads sixteen channels over all banks), B and C by
+// row.  The chunk is swept once forward, keeping the state at every eighth row, and then eight rows at a time
+// from its end: forward again with all eight states and decays in registers, and back over them.
 //   g = C dy + G;  dC = dy h;  dB = d u g;  G = a g;  w = G h_before;  dA += d w;
 //   du = d sum(g B) + D dy;  dd = u sum(g B) + sum(A w)
-// Sums over n stay in the LPC lanes of a channel; dB and dC are summed over the channels of the wavefront
-// (v_permlane swaps halve eight values to two, then rotations within a row of lanes), over the four
+// Eight rows without the start or end of a sequence (nearly all) run without a branch, so that LDS and exp
+// latencies overlap.  Sums over n stay in the LPC lanes of a channel; dB and dC are summed over the channels of the
+// wavefront (v_permlane swaps halve eight values to two, then rotations within a row of lanes), over the four
 // wavefronts in LDS, and over the workgroups of a group by k_scan_reduce: a fixed order throughout.
 constexpr int SUB = 8;
 
@@ -312,17 +440,34 @@ __device__ __forceinline__ float sum_channels(float v) {     // over the lanes o
     return v;
 }
 
+// Eight neighbouring elements in LDS, 16 bytes aligned.
+template <typename M>
+__device__ __forceinline__ void read8(float (&v)[SUB], const M* p) {
+    struct alignas(16) Eight { M e[SUB]; };
+    const Eight q = *reinterpret_cast<const Eight*>(p);
+#pragma unroll
+    for (int j = 0; j < SUB; ++j) v[j] = widen(q.e[j]);
+}
+template <typename M>
+__device__ __forceinline__ void write8(M* p, const float (&v)[SUB]) {
+    struct alignas(16) Eight { M e[SUB]; } q;
+#pragma unroll
+    for (int j = 0; j < SUB; ++j) q.e[j] = narrow<M>(v[j]);
+    *reinterpret_cast<Eight*>(p) = q;
+}
+
 template <typename T, int NP>
 __global__ __launch_bounds__(256) void k_scan_bwd(const Scan a) {
     using M = typename T::mem;
     constexpr int LPC = bwd_lpc<NP>(), CPW = WAVE / LPC, CPB = 4 * CPW, MAXR = bwd_rows<NP>(), NSUB = MAXR / SUB;
-    __shared__ float sd[MAXR * CPB];                 // d, later the gradient of d
-    __shared__ M su[MAXR * CPB];                     // u, later its gradient
-    __shared__ M sdy[MAXR * CPB];
-    __shared__ float sB[MAXR * NP], sC[MAXR * NP];
-    __shared__ float slab[4][SUB][2][NP];
-    __shared__ int sseq[MAXR], sflag[MAXR];
-    __shared__ float ssum[256];
+    constexpr int SD = MAXR + 4, SM = MAXR + 16 / (int)sizeof(M);      // distance between channels
+    constexpr int QUADS = CPB / 4, PASS_ROWS = 256 / QUADS, PASSES = MAXR / PASS_ROWS;   // staging: four channels a thread
+    __shared__ alignas(16) float sd[CPB * SD];           // d, later the gradient of d
+    __shared__ alignas(16) M su[CPB * SM];               // u, later its gradient
+    __shared__ alignas(16) M sdy[CPB * SM];
+    __shared__ alignas(16) float sB[MAXR * NP], sC[MAXR * NP];
+    __shared__ alignas(16) float slab[4 * SUB * 2 * NP > PASS_ROWS * CPB ? 4 * SUB * 2 * NP : PASS_ROWS * CPB];
+    __shared__ int sseq[WAVE], sflag[WAVE];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int n_blocks = a.groups * a.blocks_per_group;
     const int cb = blockIdx.x % n_blocks, k = blockIdx.x / n_blocks;
@@ -330,43 +475,64 @@ __global__ __launch_bounds__(256) void k_scan_bwd(const Scan a) {
     const int64_t r0 = (int64_t)k * a.chunk;
     const int len = (int)min((int64_t)a.chunk, a.rows - r0);
     const int c_base = g * a.per + gb * CPB, n_ch = min(a.per - gb * CPB, CPB);
-    enum { OUT = 4, START = 1, END = 2 };
+    enum { OUT = 4, START = 1, END = 2, NONE = 8 };
 
-    if (tid < len) {
-        const Place q = find_row(a.off, a.n_seqs, a.rows, r0 + tid);
-        sseq[tid] = q.s;
-        sflag[tid] = !q.inside ? (OUT | START | END)
-                               : (r0 + tid == q.start ? START : 0) | (r0 + tid + 1 == q.end ? END : 0);
+    if (tid < WAVE) {
+        int flag = NONE;
+        if (tid < len) {
+            const Place q = find_row(a.off, a.n_seqs, a.rows, r0 + tid);
+            sseq[tid] = q.s;
+            flag = !q.inside ? (OUT | START | END)
+                             : (r0 + tid == q.start ? START : 0) | (r0 + tid + 1 == q.end ? END : 0);
+        }
+        sflag[tid] = flag;
     }
     __syncthreads();
-    {   // rows outside every sequence count as zero, whatever they hold
-        const int ch = tid % CPB;
-        const float bias = a.bias && ch < n_ch ? a.bias[c_base + ch] : 0.0f;
-        float dD = 0.0f;
-        for (int t = tid / CPB; t < len; t += 256 / CPB) {
-            float d = 0.0f; M uv = (M)0.0f, dv = (M)0.0f;
-            if (ch < n_ch && !(sflag[t] & OUT)) {
-                const int64_t row = r0 + t;
-                d = step_of(a, static_cast<const M*>(a.delta)[row * a.delta_stride + c_base + ch], bias);
-                uv = static_cast<const M*>(a.u)[row * a.u_stride + c_base + ch];
-                dv = static_cast<const M*>(a.dy)[row * a.dy_stride + c_base + ch];
-                dD = fmaf(widen(uv), widen(dv), dD);
-            }
-            sd[t * CPB + ch] = d; su[t * CPB + ch] = uv; sdy[t * CPB + ch] = dv;
+    const int sq = (tid % QUADS) * 4, srow = tid / QUADS, s_n = max(n_ch - sq, 0);      // the thread's channels and row
+    // sums over the rows of a value per channel, from the threads' shares
+    auto fold = [&](const float (&v)[4], float* part) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) slab[srow * CPB + sq + i] = v[i];
+        __syncthreads();
+        if (part && tid < n_ch) {
+            float s = 0.0f;
+            for (int i = 0; i < PASS_ROWS; ++i) s += slab[i * CPB + tid];
+            part[(int64_t)k * a.channels + c_base + tid] = s;
         }
-        ssum[tid] = dD;
+    };
+    {   // rows outside every sequence count as zero, whatever they hold
+        float raw[PASSES][4], uv[PASSES][4], dv[PASSES][4], bias[4], dD[4] = {};
+#pragma unroll
+        for (int p = 0; p < PASSES; ++p) {
+            const int64_t row = r0 + min(p * PASS_ROWS + srow, len - 1);
+            load_vec<M, 4>(raw[p], static_cast<const M*>(a.delta) + row * a.delta_stride + c_base + sq, s_n);
+            load_vec<M, 4>(uv[p], static_cast<const M*>(a.u) + row * a.u_stride + c_base + sq, s_n);
+            load_vec<M, 4>(dv[p], static_cast<const M*>(a.dy) + row * a.dy_stride + c_base + sq, s_n);
+        }
+        load_vec<float, 4>(bias, a.bias + c_base + sq, a.bias ? s_n : 0);
         for (int i = tid; i < len * NP; i += 256) {
             const int t = i / NP, n = i % NP;
             const bool in = n < a.state && !(sflag[t] & OUT);
             sB[i] = in ? widen(static_cast<const M*>(a.B)[(r0 + t) * a.B_stride + (int64_t)g * a.state + n]) : 0.0f;
             sC[i] = in ? widen(static_cast<const M*>(a.C)[(r0 + t) * a.C_stride + (int64_t)g * a.state + n]) : 0.0f;
         }
-        __syncthreads();
-        if (a.part_D && tid < n_ch) {
-            float s = 0.0f;
-            for (int i = tid; i < 256; i += CPB) s += ssum[i];
-            a.part_D[(int64_t)k * a.channels + c_base + tid] = s;
+#pragma unroll
+        for (int p = 0; p < PASSES; ++p) {
+            const int t = p * PASS_ROWS + srow;
+            const bool in = t < len && !(sflag[t] & OUT);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const bool has = in && i < s_n;
+                const float d = has ? step_of(a.softplus, narrow<M>(raw[p][i]), bias[i]) : 0.0f;
+                const float x = has ? uv[p][i] : 0.0f, y = has ? dv[p][i] : 0.0f;
+                dD[i] = fmaf(x, y, dD[i]);
+                sd[(sq + i) * SD + t] = d;
+                su[(sq + i) * SM + t] = narrow<M>(x);
+                sdy[(sq + i) * SM + t] = narrow<M>(y);
+            }
         }
+        fold(dD, a.part_D);
     }
 
     const int nq = lane % LPC, chl = wave * CPW + lane / LPC;       // the lane's states and channel
@@ -384,166 +550,221 @@ __global__ __launch_bounds__(256) void k_scan_bwd(const Scan a) {
         G[i] = has ? a.gst[at] : 0.0f;
         dA[i] = 0.0f;
     }
-    auto enter = [&](float (&v)[4], int t, const float* from) {       // a state of the sequence of row t
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            v[i] = from && live && !(sflag[t] & OUT) && n0 + i < a.state
-                       ? from[((int64_t)sseq[t] * a.channels + c) * a.state + n0 + i] : 0.0f;
+    const int n_left = live ? max(a.state - n0, 0) : 0;
+    auto enter = [&](float (&v)[4], int t, int flag, const float* from) {       // a state of the sequence of row t
+        load_vec<float, 4>(v, from + ((int64_t)sseq[t] * a.channels + c) * a.state + n0, from && !(flag & OUT) ? n_left : 0);
     };
-    auto four = [&](const float* p) { return *reinterpret_cast<const float4*>(p); };
+    auto four = [&](float (&v)[4], const float* p) {
+        const float4 q = *reinterpret_cast<const float4*>(p);
+        v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+    };
+    // eight rows of d and u of the lane's channel
+    float* const pd = sd + chl * SD;
+    M* const pu = su + chl * SM;
+    M* const pdy = sdy + chl * SM;
+    const uint64_t marked = __ballot(sflag[lane] != 0);
+    auto flag_at = [&](int t) { return __builtin_amdgcn_readfirstlane(sflag[t]); };
 
     const int n_sub = (len + SUB - 1) / SUB;
     float keep[NSUB][4];
-#pragma unroll
-    for (int s = 0; s < NSUB; ++s) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) keep[s][i] = h[i];
-        if (s + 1 < n_sub) {
-#pragma unroll
-            for (int j = 0; j < SUB; ++j) {
-                const int t = s * SUB + j;
-                if (__builtin_amdgcn_readfirstlane(sflag[t]) & START) enter(h, t, a.initial);
-                const float d = sd[t * CPB + chl], du = d * widen(su[t * CPB + chl]);
-                const float4 b = four(sB + t * NP + n0);
-                h[0] = fmaf(exp2_hw(d * A2[0]), h[0], du * b.x);
-                h[1] = fmaf(exp2_hw(d * A2[1]), h[1], du * b.y);
-                h[2] = fmaf(exp2_hw(d * A2[2]), h[2], du * b.z);
-                h[3] = fmaf(exp2_hw(d * A2[3]), h[3], du * b.w);
-            }
-        }
-    }
-#pragma unroll
-    for (int s = NSUB - 1; s >= 0; --s) {
-        if (s >= n_sub) continue;
-        float hs[SUB + 1][4], ea[SUB][4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) hs[0][i] = keep[s][i];
+    auto sweep = [&](auto plain, int s) {
+        float d[SUB], uv[SUB];
+        read8(d, pd + s * SUB);
+        read8(uv, pu + s * SUB);
 #pragma unroll
         for (int j = 0; j < SUB; ++j) {
             const int t = s * SUB + j;
-            if (t < len) {
-                float prev[4];
+            if (!decltype(plain)::value) {
+                const int flag = flag_at(t);
+                if (flag & START) enter(h, t, flag, a.initial);
+            }
+            float b[4];
+            four(b, sB + t * NP + n0);
+            const float du = d[j] * uv[j];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) prev[i] = hs[j][i];
-                if (__builtin_amdgcn_readfirstlane(sflag[t]) & START) enter(prev, t, a.initial);
-                const float d = sd[t * CPB + chl], du = d * widen(su[t * CPB + chl]);
-                const float4 b4 = four(sB + t * NP + n0);
-                const float b[4] = {b4.x, b4.y, b4.z, b4.w};
+            for (int i = 0; i < 4; ++i) h[i] = fmaf(exp2_hw(d[j] * A2[i]), h[i], du * b[i]);
+        }
+    };
+    for (int s = 0; s < n_sub; ++s) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    ea[j][i] = exp2_hw(d * A2[i]);
-                    hs[j + 1][i] = fmaf(ea[j][i], prev[i], du * b[i]);
+        for (int q = 0; q < NSUB; ++q)
+            if (q == s) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) keep[q][i] = h[i];
+            }
+        if (s + 1 == n_sub) break;
+        if ((marked >> (s * SUB)) & 0xff) sweep(std::false_type{}, s);
+        else sweep(std::true_type{}, s);
+    }
+
+    auto back = [&](auto plain, int s) {
+        constexpr bool PLAIN = decltype(plain)::value;
+        float d[SUB], uv[SUB], dv[SUB], hs[SUB + 1][4], ea[SUB][4], dd[SUB], gu[SUB];
+        read8(d, pd + s * SUB);
+        read8(uv, pu + s * SUB);
+        read8(dv, pdy + s * SUB);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) hs[0][i] = h[i];
+#pragma unroll
+        for (int j = 0; j < SUB; ++j) {
+            const int t = s * SUB + j;
+            float prev[4], b[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) prev[i] = hs[j][i];
+            if (!PLAIN) {
+                const int flag = flag_at(t);
+                if (flag & NONE) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) { ea[j][i] = 1.0f; hs[j + 1][i] = 0.0f; }
+                    continue;
                 }
-            } else {
+                if (flag & START) enter(prev, t, flag, a.initial);
+            }
+            four(b, sB + t * NP + n0);
+            const float du = d[j] * uv[j];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) { ea[j][i] = 1.0f; hs[j + 1][i] = 0.0f; }
+            for (int i = 0; i < 4; ++i) {
+                ea[j][i] = exp2_hw(d[j] * A2[i]);
+                hs[j + 1][i] = fmaf(ea[j][i], prev[i], du * b[i]);
             }
         }
 #pragma unroll
         for (int j = SUB - 1; j >= 0; --j) {
             const int t = s * SUB + j;
-            float red[8];
-            if (t < len) {
-                const int flag = __builtin_amdgcn_readfirstlane(sflag[t]);
-                float prev[4];
+            float prev[4], b[4], cc[4], red[8];
+            dd[j] = gu[j] = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) prev[i] = hs[j][i];
-                if (flag & START) enter(prev, t, a.initial);
-                if (flag & END) enter(G, t, a.dfinal);
-                const float d = sd[t * CPB + chl], uv = widen(su[t * CPB + chl]), dv = widen(sdy[t * CPB + chl]);
-                const float du = d * uv;
-                const float4 b4 = four(sB + t * NP + n0), c4 = four(sC + t * NP + n0);
-                const float b[4] = {b4.x, b4.y, b4.z, b4.w}, cc[4] = {c4.x, c4.y, c4.z, c4.w};
-                float gB = 0.0f, wA = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float gr = fmaf(cc[i], dv, G[i]);
-                    red[i] = du * gr;
-                    red[4 + i] = dv * hs[j + 1][i];
-                    gB = fmaf(gr, b[i], gB);
-                    G[i] = ea[j][i] * gr;
-                    const float w = G[i] * prev[i];
-                    dA[i] = fmaf(d, w, dA[i]);
-                    wA = fmaf(A[i], w, wA);
-                }
-                if ((flag & START) && a.dinitial && !(flag & OUT) && live) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (n0 + i < a.state) a.dinitial[((int64_t)sseq[t] * a.channels + c) * a.state + n0 + i] = G[i];
-                }
-                gB = sum_states<LPC>(gB);
-                wA = sum_states<LPC>(wA);
-                if (nq == 0) {
-                    sd[t * CPB + chl] = fmaf(uv, gB, wA);
-                    su[t * CPB + chl] = narrow<M>(fmaf(d, gB, skip * dv));
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) red[i] = 0.0f;
+            for (int i = 0; i < 4; ++i) prev[i] = hs[j][i];
+            int flag = 0;
+            if (!PLAIN) {
+                flag = flag_at(t);
+                if (flag & NONE) continue;
+                if (flag & START) enter(prev, t, flag, a.initial);
+                if (flag & END) enter(G, t, flag, a.dfinal);
             }
+            four(b, sB + t * NP + n0);
+            four(cc, sC + t * NP + n0);
+            const float du = d[j] * uv[j];
+            float gB = 0.0f, wA = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float gr = fmaf(cc[i], dv[j], G[i]);
+                red[i] = du * gr;
+                red[4 + i] = dv[j] * hs[j + 1][i];
+                gB = fmaf(gr, b[i], gB);
+                G[i] = ea[j][i] * gr;
+                const float w = G[i] * prev[i];
+                dA[i] = fmaf(d[j], w, dA[i]);
+                wA = fmaf(A[i], w, wA);
+            }
+            if (!PLAIN && (flag & START) && a.dinitial && !(flag & OUT) && n_left > 0)
+                store_vec<float, 4>(a.dinitial + ((int64_t)sseq[t] * a.channels + c) * a.state + n0, G, n_left);
+            gB = sum_states<LPC>(gB);
+            wA = sum_states<LPC>(wA);
+            dd[j] = fmaf(uv[j], gB, wA);
+            gu[j] = fmaf(d[j], gB, skip * dv[j]);
             const float w0 = halve32(red[0], red[4]), w1 = halve32(red[1], red[5]);
             const float w2 = halve32(red[2], red[6]), w3 = halve32(red[3], red[7]);
             const float v0 = sum_channels<LPC>(halve16(w0, w2)), v1 = sum_channels<LPC>(halve16(w1, w3));
-            if ((lane & 15) < LPC) {
-                float* p = &slab[wave][j][lane >> 5][(lane & 15) * 4 + ((lane >> 4) & 1) * 2];
-                p[0] = v0; p[1] = v1;
-            }
+            if ((lane & 15) < LPC)
+                *reinterpret_cast<float2*>(slab + ((wave * SUB + j) * 2 + (lane >> 5)) * NP + (lane & 15) * 4 + ((lane >> 4) & 1) * 2) =
+                    make_float2(v0, v1);
         }
+        if (nq == 0) {
+            write8(pd + s * SUB, dd);
+            write8(pu + s * SUB, gu);
+        }
+    };
+    for (int s = n_sub - 1; s >= 0; --s) {
+#pragma unroll
+        for (int q = 0; q < NSUB; ++q)
+            if (q == s) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) h[i] = keep[q][i];
+            }
+        __syncthreads();
+        if ((marked >> (s * SUB)) & 0xff) back(std::false_type{}, s);
+        else back(std::true_type{}, s);
         __syncthreads();
         for (int i = tid; i < SUB * 2 * NP; i += 256) {
             const int j = i / (2 * NP), w = i / NP & 1, n = i % NP, t = s * SUB + j;
             if (t < len)
                 a.part_bc[(((int64_t)w * a.blocks_per_group + gb) * a.rows + r0 + t) * a.groups * NP + (int64_t)g * NP + n] =
-                    (slab[0][j][w][n] + slab[1][j][w][n]) + (slab[2][j][w][n] + slab[3][j][w][n]);
+                    (slab[i] + slab[SUB * 2 * NP + i]) + (slab[2 * SUB * 2 * NP + i] + slab[3 * SUB * 2 * NP + i]);
         }
-        __syncthreads();
     }
-    if (live) {
-        float* p = a.part_A + ((int64_t)k * a.channels + c) * NP + n0;
+    if (live) store_vec<float, 4>(a.part_A + ((int64_t)k * a.channels + c) * NP + n0, dA, 4);
+    __syncthreads();
+    float raw[PASSES][4], bias[4], db[4] = {};
+    if (a.softplus) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) p[i] = dA[i];
+        for (int p = 0; p < PASSES; ++p)
+            load_vec<M, 4>(raw[p], static_cast<const M*>(a.delta) + (r0 + min(p * PASS_ROWS + srow, len - 1)) * a.delta_stride + c_base + sq, s_n);
+        load_vec<float, 4>(bias, a.bias + c_base + sq, a.bias ? s_n : 0);
     }
-    __syncthreads();
-    const int ch = tid % CPB;
-    float db = 0.0f;
-    if (ch < n_ch) {
-        const float bias = a.bias ? a.bias[c_base + ch] : 0.0f;
-        for (int t = tid / CPB; t < len; t += 256 / CPB) {
-            const int64_t at = (r0 + t) * a.channels + c_base + ch;
-            float v = sd[t * CPB + ch];
-            if (sflag[t] & OUT) v = 0.0f;
-            else if (a.softplus) v *= sigmoid_f(widen(static_cast<const M*>(a.delta)[(r0 + t) * a.delta_stride + c_base + ch]) + bias);
-            db += v;
-            static_cast<M*>(a.ddelta)[at] = narrow<M>(v);
-            static_cast<M*>(a.du)[at] = su[t * CPB + ch];
+#pragma unroll
+    for (int p = 0; p < PASSES; ++p) {
+        const int t = p * PASS_ROWS + srow;
+        if (t < len && s_n > 0) {
+            float v[4], x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[i] = sd[(sq + i) * SD + t];
+                x[i] = widen(su[(sq + i) * SM + t]);
+                if (sflag[t] & OUT) v[i] = 0.0f;
+                else if (a.softplus) v[i] *= sigmoid_f(raw[p][i] + bias[i]);
+                db[i] += v[i];
+            }
+            const int64_t at = (r0 + t) * a.channels + c_base + sq;
+            store_vec<M, 4>(static_cast<M*>(a.ddelta) + at, v, s_n);
+            store_vec<M, 4>(static_cast<M*>(a.du) + at, x, s_n);
         }
     }
-    ssum[tid] = db;
-    __syncthreads();
-    if (a.part_bias && tid < n_ch) {
-        float s = 0.0f;
-        for (int i = tid; i < 256; i += CPB) s += ssum[i];
-        a.part_bias[(int64_t)k * a.channels + c_base + tid] = s;
-    }
+    if (a.part_bias) fold(db, a.part_bias);
 }
 
-// out[e] = sum over parts of part[p][e]; rows of `padded` columns of which the first `inner` are kept.
-template <typename M, typename T>
-__global__ __launch_bounds__(256) void k_scan_reduce(const float* __restrict__ part, int64_t n_part, int64_t m, int padded,
-                                                     int inner, M* __restrict__ out) {
-    __shared__ float sh[4][64];
+// The sums of the partial results, one launch for all of them: out[e] = sum over parts of part[p][e], of rows of
+// `padded` columns of which the first `inner` are kept.  64 elements by 16 slices of the parts.
+struct ReduceJob {
+    const float* part; void* out;
+    int64_t n_part, m, first_block;
+    int padded, inner, wide;             // wide: out is float32, else of the element type
+};
+struct ReduceJobs { ReduceJob job[5]; int count; };
+
+template <typename T>
+__global__ __launch_bounds__(1024) void k_scan_reduce(const ReduceJobs jobs) {
+    using M = typename T::mem;
+    __shared__ float sh[16][64];
+    int which = 0;
+    for (int i = 1; i < jobs.count; ++i)
+        if (blockIdx.x >= jobs.job[i].first_block) which = i;
+    const ReduceJob& job = jobs.job[which];
     const int lane = threadIdx.x & 63, slice = threadIdx.x >> 6;
-    for (int64_t e0 = (int64_t)blockIdx.x * 64; e0 < m; e0 += (int64_t)gridDim.x * 64) {
-        const int64_t e = e0 + lane;
-        float s = 0.0f;
-        if (e < m)
-            for (int64_t p = slice; p < n_part; p += 4) s += part[p * m + e];
+    // few parts: the slices take different elements instead
+    const bool few = job.n_part < 64;
+    const int64_t e = ((int64_t)blockIdx.x - job.first_block) * (few ? 1024 : 64) + (few ? threadIdx.x : lane);
+    float s = 0.0f;
+    if (e < job.m) {
+        const float* p = job.part + e;
+        const int step = few ? 1 : 16;
+        int64_t i = few ? 0 : slice;
+        for (; i + 3 * step < job.n_part; i += 4 * step)
+            s += (p[i * job.m] + p[(i + step) * job.m]) + (p[(i + 2 * step) * job.m] + p[(i + 3 * step) * job.m]);
+        for (; i < job.n_part; i += step) s += p[i * job.m];
+    }
+    if (!few) {
         sh[slice][lane] = s;
         __syncthreads();
-        if (slice == 0 && e < m && e % padded < inner)
-            out[e / padded * inner + e % padded] = narrow<M>((sh[0][lane] + sh[1][lane]) + (sh[2][lane] + sh[3][lane]));
-        __syncthreads();
+        if (slice) return;
+        s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s += sh[i][lane];
     }
+    if (e >= job.m || e % job.padded >= job.inner) return;
+    const int64_t at = e / job.padded * job.inner + e % job.padded;
+    if (job.wide) static_cast<float*>(job.out)[at] = s;
+    else static_cast<M*>(job.out)[at] = narrow<M>(s);
 }
 
 // ---- single tokens --------------------------------------------------------------------------------------
@@ -597,8 +818,7 @@ __global__ __launch_bounds__(256) void k_scan_step(const ScanStep a) {
             if (a.slots[e] != slot) continue;
         }
         const float uv = widen(static_cast<const M*>(a.u)[(int64_t)e * a.u_stride + c]);
-        float d = widen(static_cast<const M*>(a.delta)[(int64_t)e * a.delta_stride + c]) + bias;
-        if (a.softplus) d = softplus_f(d);
+        const float d = step_of(a.softplus, static_cast<const M*>(a.delta)[(int64_t)e * a.delta_stride + c], bias);
         float b[4], cc[4];
         load_vec<M, 4>(b, static_cast<const M*>(a.B) + (int64_t)e * a.B_stride + bc, left);
         load_vec<M, 4>(cc, static_cast<const M*>(a.C) + (int64_t)e * a.C_stride + bc, left);
@@ -756,17 +976,20 @@ int scan_backward(const mfcc_scan_args* a, hipStream_t st) {
             PACKED_LAUNCHED();
         }
         const int64_t m = a->rows * f.groups * NP;
-        auto reduce = [&](const float* part, int64_t n_part, int64_t size, int padded, int inner, auto* out) {
-            using O = std::remove_pointer_t<decltype(out)>;
-            if (size == 0) return;
-            const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(size, 64), 1 << 20);
-            hipLaunchKernelGGL((k_scan_reduce<O, T>), dim3(blocks), dim3(256), 0, st, part, n_part, size, padded, inner, out);
+        ReduceJobs jobs = {};
+        int64_t blocks = 0;
+        auto reduce = [&](const float* part, int64_t n_part, int64_t size, int padded, int inner, void* out, bool wide) {
+            if (size == 0 || !out) return;
+            jobs.job[jobs.count++] = {part, out, n_part, size, blocks, padded, inner, wide};
+            blocks += ceil_div(size, n_part < 64 ? 1024 : 64);
         };
-        reduce(f.part_bc, f.blocks_per_group, m, NP, f.state, static_cast<M*>(a->d_dB));
-        reduce(f.part_bc + f.blocks_per_group * m, f.blocks_per_group, m, NP, f.state, static_cast<M*>(a->d_dC));
-        reduce(f.part_A, f.n_chunks, (int64_t)f.channels * NP, NP, f.state, a->d_dA);
-        if (a->d_dD) reduce(f.part_D, f.n_chunks, f.channels, 1, 1, a->d_dD);
-        if (a->d_ddelta_bias) reduce(f.part_bias, f.n_chunks, f.channels, 1, 1, a->d_ddelta_bias);
+        reduce(f.part_bc, f.blocks_per_group, m, NP, f.state, a->d_dB, sizeof(M) == 4);
+        reduce(f.part_bc + f.blocks_per_group * m, f.blocks_per_group, m, NP, f.state, a->d_dC, sizeof(M) == 4);
+        reduce(f.part_A, f.n_chunks, (int64_t)f.channels * NP, NP, f.state, a->d_dA, true);
+        reduce(f.part_D, f.n_chunks, f.channels, 1, 1, a->d_dD, true);
+        reduce(f.part_bias, f.n_chunks, f.channels, 1, 1, a->d_ddelta_bias, true);
+        if (blocks > 0x3fffff) return mfcc_detail::fail(MFCC_E_UNSUPPORTED, "batch too large: split it");
+        hipLaunchKernelGGL(k_scan_reduce<T>, dim3((unsigned)blocks), dim3(1024), 0, st, jobs);
         PACKED_LAUNCHED();
         return scan_empties<T>(a, a->d_dfinal, a->d_dinitial, st);
     });
