@@ -90,7 +90,12 @@ __device__ __forceinline__ float exp_f(float x) {
     return fabsf(p) < 126.0f ? fmaf(e * LN2, lo, e) : e;
 }
 
-__device__ __forceinline__ float sigmoid_f(float x) { return rcp_hw(1.0f + exp_f(-x)); }
+// EXACT = false leaves out the second float of the exponent's product: |x| 2^-24 more, for results or
+// arguments that are rounded to 16 bits anyway.
+template <bool EXACT = true>
+__device__ __forceinline__ float sigmoid_f(float x) {
+    return rcp_hw(1.0f + (EXACT ? exp_f(-x) : exp2_hw(x * -LOG2E)));
+}
 
 // log(1 + exp(x)) = max(x, 0) + log(1 + e), e = exp(-|x|) in (0, 1].  w = 1 + e loses the low bits of a
 // small e; what it lost, e - (w - 1), is exact and is added back (to first order: the error of that is

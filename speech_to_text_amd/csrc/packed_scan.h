@@ -422,6 +422,10 @@ template <int NP> constexpr int bwd_lpc() { return NP / 4; }
 template <int NP> constexpr int bwd_channels() { return 4 * WAVE / bwd_lpc<NP>(); }
 template <int NP> constexpr int bwd_rows() { return bwd_channels<NP>() >= 256 ? 16 : bwd_channels<NP>() >= 128 ? 32 : 64; }
 
+// Wavefronts per SIMD that the LDS of the gradient kernel allows; held to three in registers too (a few spilled
+// around the rare paths) it is 8 % faster than with two.
+template <typename T, int NP> constexpr int bwd_waves() { return sizeof(typename T::mem) == 2 && NP >= 16 ? 3 : 2; }
+
 template <int LPC>
 __device__ __forceinline__ float sum_states(float v) {       // over the LPC neighbouring lanes of a channel
     if (LPC >= 2) v += dpp<0xB1>(v);                          // quad_perm [1, 0, 3, 2]
@@ -440,24 +444,11 @@ __device__ __forceinline__ float sum_channels(float v) {     // over the lanes o
     return v;
 }
 
-// Eight neighbouring elements in LDS, 16 bytes aligned.
-template <typename M>
-__device__ __forceinline__ void read8(float (&v)[SUB], const M* p) {
-    struct alignas(16) Eight { M e[SUB]; };
-    const Eight q = *reinterpret_cast<const Eight*>(p);
-#pragma unroll
-    for (int j = 0; j < SUB; ++j) v[j] = widen(q.e[j]);
-}
-template <typename M>
-__device__ __forceinline__ void write8(M* p, const float (&v)[SUB]) {
-    struct alignas(16) Eight { M e[SUB]; } q;
-#pragma unroll
-    for (int j = 0; j < SUB; ++j) q.e[j] = narrow<M>(v[j]);
-    *reinterpret_cast<Eight*>(p) = q;
-}
+// Eight neighbouring elements in LDS, 16 bytes aligned; left in their type (the registers) until they are used.
+template <typename M> struct alignas(16) Eight { M e[SUB]; };
 
 template <typename T, int NP>
-__global__ __launch_bounds__(256) void k_scan_bwd(const Scan a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(bwd_waves<T, NP>()))) void k_scan_bwd(const Scan a) {
     using M = typename T::mem;
     constexpr int LPC = bwd_lpc<NP>(), CPW = WAVE / LPC, CPB = 4 * CPW, MAXR = bwd_rows<NP>(), NSUB = MAXR / SUB;
     constexpr int SD = MAXR + 4, SM = MAXR + 16 / (int)sizeof(M);      // distance between channels
@@ -466,7 +457,8 @@ __global__ __launch_bounds__(256) void k_scan_bwd(const Scan a) {
     __shared__ alignas(16) M su[CPB * SM];               // u, later its gradient
     __shared__ alignas(16) M sdy[CPB * SM];
     __shared__ alignas(16) float sB[MAXR * NP], sC[MAXR * NP];
-    __shared__ alignas(16) float slab[4 * SUB * 2 * NP > PASS_ROWS * CPB ? 4 * SUB * 2 * NP : PASS_ROWS * CPB];
+    constexpr int SLAB = 4 * SUB * 2 * NP;               // eight rows of dB and dC from each wavefront, twice
+    __shared__ alignas(16) float slab[2 * SLAB > PASS_ROWS * CPB ? 2 * SLAB : PASS_ROWS * CPB];
     __shared__ int sseq[WAVE], sflag[WAVE];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int n_blocks = a.groups * a.blocks_per_group;
@@ -500,6 +492,7 @@ __global__ __launch_bounds__(256) void k_scan_bwd(const Scan a) {
             for (int i = 0; i < PASS_ROWS; ++i) s += slab[i * CPB + tid];
             part[(int64_t)k * a.channels + c_base + tid] = s;
         }
+        __syncthreads();
     };
     {   // rows outside every sequence count as zero, whatever they hold
         float raw[PASSES][4], uv[PASSES][4], dv[PASSES][4], bias[4], dD[4] = {};
@@ -511,11 +504,13 @@ __global__ __launch_bounds__(256) void k_scan_bwd(const Scan a) {
             load_vec<M, 4>(dv[p], static_cast<const M*>(a.dy) + row * a.dy_stride + c_base + sq, s_n);
         }
         load_vec<float, 4>(bias, a.bias + c_base + sq, a.bias ? s_n : 0);
-        for (int i = tid; i < len * NP; i += 256) {
-            const int t = i / NP, n = i % NP;
-            const bool in = n < a.state && !(sflag[t] & OUT);
-            sB[i] = in ? widen(static_cast<const M*>(a.B)[(r0 + t) * a.B_stride + (int64_t)g * a.state + n]) : 0.0f;
-            sC[i] = in ? widen(static_cast<const M*>(a.C)[(r0 + t) * a.C_stride + (int64_t)g * a.state + n]) : 0.0f;
+        for (int i = tid; i < len * LPC; i += 256) {
+            const int t = i / LPC, n = i % LPC * 4, count = sflag[t] & OUT ? 0 : max(a.state - n, 0);
+            float b[4], cc[4];
+            load_vec<M, 4>(b, static_cast<const M*>(a.B) + (r0 + t) * a.B_stride + (int64_t)g * a.state + n, count);
+            load_vec<M, 4>(cc, static_cast<const M*>(a.C) + (r0 + t) * a.C_stride + (int64_t)g * a.state + n, count);
+            *reinterpret_cast<float4*>(sB + i * 4) = make_float4(b[0], b[1], b[2], b[3]);
+            *reinterpret_cast<float4*>(sC + i * 4) = make_float4(cc[0], cc[1], cc[2], cc[3]);
         }
 #pragma unroll
         for (int p = 0; p < PASSES; ++p) {
@@ -539,11 +534,10 @@ __global__ __launch_bounds__(256) void k_scan_bwd(const Scan a) {
     const bool live = chl < n_ch;
     const int c = c_base + (live ? chl : 0), n0 = nq * 4;
     const float skip = a.D ? a.D[c] : 0.0f;
-    float A[4], A2[4], h[4], G[4], dA[4];
+    float A2[4], h[4], G[4], dA[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        A[i] = n0 + i < a.state ? a.A[(int64_t)c * a.state + n0 + i] : 0.0f;
-        A2[i] = A[i] * SCAN_LOG2E;
+        A2[i] = n0 + i < a.state ? a.A[(int64_t)c * a.state + n0 + i] * SCAN_LOG2E : 0.0f;
         const bool has = a.n_chunks > 1 && live && n0 + i < a.state;
         const int64_t at = ((int64_t)k * a.state + n0 + i) * a.channels + c;
         h[i] = has ? a.hst[at] : 0.0f;
@@ -562,15 +556,16 @@ __global__ __launch_bounds__(256) void k_scan_bwd(const Scan a) {
     float* const pd = sd + chl * SD;
     M* const pu = su + chl * SM;
     M* const pdy = sdy + chl * SM;
+    float* const pslab = slab + (wave * SUB * 2 + (lane >> 5)) * NP + n0 + ((lane >> 4) & 1) * 2;
     const uint64_t marked = __ballot(sflag[lane] != 0);
     auto flag_at = [&](int t) { return __builtin_amdgcn_readfirstlane(sflag[t]); };
 
     const int n_sub = (len + SUB - 1) / SUB;
     float keep[NSUB][4];
     auto sweep = [&](auto plain, int s) {
-        float d[SUB], uv[SUB];
-        read8(d, pd + s * SUB);
-        read8(uv, pu + s * SUB);
+        const Eight<float> d8 = *reinterpret_cast<const Eight<float>*>(pd + s * SUB);
+        const Eight<M> u8 = *reinterpret_cast<const Eight<M>*>(pu + s * SUB);
+        const float* pB = sB + s * SUB * NP + n0;
 #pragma unroll
         for (int j = 0; j < SUB; ++j) {
             const int t = s * SUB + j;
@@ -579,10 +574,10 @@ __global__ __launch_bounds__(256) void k_scan_bwd(const Scan a) {
                 if (flag & START) enter(h, t, flag, a.initial);
             }
             float b[4];
-            four(b, sB + t * NP + n0);
-            const float du = d[j] * uv[j];
+            four(b, pB + j * NP);
+            const float d = d8.e[j], du = d * widen(u8.e[j]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) h[i] = fmaf(exp2_hw(d[j] * A2[i]), h[i], du * b[i]);
+            for (int i = 0; i < 4; ++i) h[i] = fmaf(exp2_hw(d * A2[i]), h[i], du * b[i]);
         }
     };
     for (int s = 0; s < n_sub; ++s) {
@@ -599,10 +594,11 @@ __global__ __launch_bounds__(256) void k_scan_bwd(const Scan a) {
 
     auto back = [&](auto plain, int s) {
         constexpr bool PLAIN = decltype(plain)::value;
-        float d[SUB], uv[SUB], dv[SUB], hs[SUB + 1][4], ea[SUB][4], dd[SUB], gu[SUB];
-        read8(d, pd + s * SUB);
-        read8(uv, pu + s * SUB);
-        read8(dv, pdy + s * SUB);
+        float hs[SUB + 1][4], ea[SUB][4];
+        Eight<float> d8 = *reinterpret_cast<const Eight<float>*>(pd + s * SUB);      // d, then its gradient
+        Eight<M> u8 = *reinterpret_cast<const Eight<M>*>(pu + s * SUB);              // u, then its gradient
+        const Eight<M> y8 = *reinterpret_cast<const Eight<M>*>(pdy + s * SUB);
+        int at = s * SUB * NP + n0;                      // of the lane's four B in the row, and C
 #pragma unroll
         for (int i = 0; i < 4; ++i) hs[0][i] = h[i];
 #pragma unroll
@@ -620,19 +616,19 @@ __global__ __launch_bounds__(256) void k_scan_bwd(const Scan a) {
                 }
                 if (flag & START) enter(prev, t, flag, a.initial);
             }
-            four(b, sB + t * NP + n0);
-            const float du = d[j] * uv[j];
+            four(b, sB + at + j * NP);
+            const float d = d8.e[j], du = d * widen(u8.e[j]);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                ea[j][i] = exp2_hw(d[j] * A2[i]);
+                ea[j][i] = exp2_hw(d * A2[i]);
                 hs[j + 1][i] = fmaf(ea[j][i], prev[i], du * b[i]);
             }
+            if (j % 2) after(at, hs[j][0]);
         }
 #pragma unroll
         for (int j = SUB - 1; j >= 0; --j) {
             const int t = s * SUB + j;
             float prev[4], b[4], cc[4], red[8];
-            dd[j] = gu[j] = 0.0f;
 #pragma unroll
             for (int i = 0; i < 4; ++i) prev[i] = hs[j][i];
             int flag = 0;
@@ -642,39 +638,42 @@ __global__ __launch_bounds__(256) void k_scan_bwd(const Scan a) {
                 if (flag & START) enter(prev, t, flag, a.initial);
                 if (flag & END) enter(G, t, flag, a.dfinal);
             }
-            four(b, sB + t * NP + n0);
-            four(cc, sC + t * NP + n0);
-            const float du = d[j] * uv[j];
+            four(b, sB + at + j * NP);
+            four(cc, sC + at + j * NP);
+            const float d = d8.e[j], uv = widen(u8.e[j]), dv = widen(y8.e[j]), du = d * uv;
             float gB = 0.0f, wA = 0.0f;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float gr = fmaf(cc[i], dv[j], G[i]);
+                const float gr = fmaf(cc[i], dv, G[i]);
                 red[i] = du * gr;
-                red[4 + i] = dv[j] * hs[j + 1][i];
+                red[4 + i] = dv * hs[j + 1][i];
                 gB = fmaf(gr, b[i], gB);
                 G[i] = ea[j][i] * gr;
                 const float w = G[i] * prev[i];
-                dA[i] = fmaf(d[j], w, dA[i]);
-                wA = fmaf(A[i], w, wA);
+                dA[i] = fmaf(d, w, dA[i]);
+                wA = fmaf(A2[i], w, wA);
             }
+            after(at, G[0]);
             if (!PLAIN && (flag & START) && a.dinitial && !(flag & OUT) && n_left > 0)
                 store_vec<float, 4>(a.dinitial + ((int64_t)sseq[t] * a.channels + c) * a.state + n0, G, n_left);
             gB = sum_states<LPC>(gB);
             wA = sum_states<LPC>(wA);
-            dd[j] = fmaf(uv[j], gB, wA);
-            gu[j] = fmaf(d[j], gB, skip * dv[j]);
+            d8.e[j] = fmaf(uv, gB, wA * LN2);              // A = A2 ln 2
+            u8.e[j] = narrow<M>(fmaf(d, gB, skip * dv));
             const float w0 = halve32(red[0], red[4]), w1 = halve32(red[1], red[5]);
             const float w2 = halve32(red[2], red[6]), w3 = halve32(red[3], red[7]);
             const float v0 = sum_channels<LPC>(halve16(w0, w2)), v1 = sum_channels<LPC>(halve16(w1, w3));
-            if ((lane & 15) < LPC)
-                *reinterpret_cast<float2*>(slab + ((wave * SUB + j) * 2 + (lane >> 5)) * NP + (lane & 15) * 4 + ((lane >> 4) & 1) * 2) =
-                    make_float2(v0, v1);
+            // all lanes of a row with the same states hold the same sums: they write one place
+            *reinterpret_cast<float2*>(pslab + (s & 1) * SLAB + j * 2 * NP) = make_float2(v0, v1);
         }
         if (nq == 0) {
-            write8(pd + s * SUB, dd);
-            write8(pu + s * SUB, gu);
+            *reinterpret_cast<Eight<float>*>(pd + s * SUB) = d8;
+            *reinterpret_cast<Eight<M>*>(pu + s * SUB) = u8;
         }
     };
+    float* const part_bc = a.part_bc + ((int64_t)gb * a.rows + r0) * a.groups * NP + (int64_t)g * NP;
+    const int64_t bc_which = (int64_t)a.blocks_per_group * a.rows * a.groups * NP;
+    const int bc_row = a.groups * NP;
     for (int s = n_sub - 1; s >= 0; --s) {
 #pragma unroll
         for (int q = 0; q < NSUB; ++q)
@@ -682,15 +681,16 @@ __global__ __launch_bounds__(256) void k_scan_bwd(const Scan a) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) h[i] = keep[q][i];
             }
-        __syncthreads();
         if ((marked >> (s * SUB)) & 0xff) back(std::false_type{}, s);
         else back(std::true_type{}, s);
-        __syncthreads();
-        for (int i = tid; i < SUB * 2 * NP; i += 256) {
-            const int j = i / (2 * NP), w = i / NP & 1, n = i % NP, t = s * SUB + j;
-            if (t < len)
-                a.part_bc[(((int64_t)w * a.blocks_per_group + gb) * a.rows + r0 + t) * a.groups * NP + (int64_t)g * NP + n] =
-                    (slab[i] + slab[SUB * 2 * NP + i]) + (slab[2 * SUB * 2 * NP + i] + slab[3 * SUB * 2 * NP + i]);
+        __syncthreads();          // one is enough: the other half of the slab is written before the next
+        const float* sum4 = slab + (s & 1) * SLAB;
+#pragma unroll
+        for (int q = 0; q < (SUB * 2 * NP + 255) / 256; ++q) {
+            const int i = q * 256 + tid, j = i / (2 * NP), w = i / NP & 1;
+            if (i < SUB * 2 * NP && s * SUB + j < len)
+                part_bc[w * bc_which + (s * SUB + j) * bc_row + i % NP] =
+                    (sum4[i] + sum4[SLAB / 4 + i]) + (sum4[SLAB / 2 + i] + sum4[3 * SLAB / 4 + i]);
         }
     }
     if (live) store_vec<float, 4>(a.part_A + ((int64_t)k * a.channels + c) * NP + n0, dA, 4);
@@ -712,7 +712,7 @@ __global__ __launch_bounds__(256) void k_scan_bwd(const Scan a) {
                 v[i] = sd[(sq + i) * SD + t];
                 x[i] = widen(su[(sq + i) * SM + t]);
                 if (sflag[t] & OUT) v[i] = 0.0f;
-                else if (a.softplus) v[i] *= sigmoid_f(raw[p][i] + bias[i]);
+                else if (a.softplus) v[i] *= sigmoid_f<sizeof(M) == 4>(raw[p][i] + bias[i]);
                 db[i] += v[i];
             }
             const int64_t at = (r0 + t) * a.channels + c_base + sq;

@@ -81,18 +81,23 @@ def _rows(t, name, like=None, dtype=None):
     """Rows of an operator: (rows, channels) on a GPU, unit stride along the channels."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ParameterError(f"{name} must be a device tensor: there is no CPU fallback")
-    if t.ndim != 2 or t.shape[1] == 0 or (t.stride(1) != 1 and t.shape[1] > 1):
+    shape = t.shape
+    if len(shape) != 2 or shape[1] == 0 or (t.stride(1) != 1 and shape[1] > 1):
         raise ParameterError(f"{name} must be (rows, channels) with unit stride along the channels, "
-                             f"got shape {tuple(t.shape)}, strides {t.stride()}")
+                             f"got shape {tuple(shape)}, strides {t.stride()}")
     if like is None:
         if t.dtype not in _DTYPE:
             raise ParameterError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
     else:
-        if t.shape != like.shape or t.device != like.device:
-            raise ParameterError(f"{name} must be {tuple(like.shape)} on {like.device}, got {tuple(t.shape)} on {t.device}")
-        if t.dtype != (dtype or like.dtype):
+        if shape != like.shape or t.get_device() != like.get_device():
+            raise ParameterError(f"{name} must be {tuple(like.shape)} on {like.device}, got {tuple(shape)} on {t.device}")
+        if t.dtype is not (dtype or like.dtype):
             raise ParameterError(f"{name} must be {dtype or like.dtype}, got {t.dtype}")
     return t
+
+
+def _described(t):
+    return f"{tuple(t.shape)} {t.dtype} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
 
 
 def _table(t, name, shape, x, optional=True):
@@ -101,18 +106,16 @@ def _table(t, name, shape, x, optional=True):
         if optional:
             return None
         raise ParameterError(f"{name} is missing")
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != x.device or tuple(t.shape) != tuple(shape):
-        got = f"{tuple(t.shape)} {t.dtype} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
-        raise ParameterError(f"{name} must be a float32 tensor of shape {tuple(shape)} on {x.device}, got {got}")
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.float32 or t.shape != shape or t.get_device() != x.get_device():
+        raise ParameterError(f"{name} must be a float32 tensor of shape {shape} on {x.device}, got {_described(t)}")
     return t if t.is_contiguous() else t.contiguous()
 
 
 def _state(t, name, shape, dtype, x, writable=False):
     if t is None:
         return None
-    if (not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != x.device or tuple(t.shape) != tuple(shape)):
-        got = f"{tuple(t.shape)} {t.dtype} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
-        raise ParameterError(f"{name} must be a {dtype} tensor of shape {tuple(shape)} on {x.device}, got {got}")
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.shape != shape or t.get_device() != x.get_device():
+        raise ParameterError(f"{name} must be a {dtype} tensor of shape {shape} on {x.device}, got {_described(t)}")
     if t.is_contiguous():
         return t
     if writable:
@@ -143,7 +146,7 @@ def _overlap(a, b) -> bool:
 def _out(out, x, inputs, dtype=None):
     """The output rows: new ones, or the caller's after a check."""
     if out is None:
-        return torch.empty(x.shape, dtype=dtype or x.dtype, device=x.device)
+        return x.new_empty(x.shape, dtype=dtype or x.dtype)
     _rows(out, "out", x, dtype)
     if out.shape[0] > 1 and out.stride(0) < out.shape[1]:
         raise ParameterError("the rows of out overlap")
@@ -179,17 +182,27 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _run(device, fn, args):
-    """fn(args, current stream) on the tensors' device."""
-    if torch.cuda.current_device() == device.index:
-        _check(fn(args, torch.cuda.current_stream().cuda_stream))
+# the handle of a device's current stream, without the Stream object torch.cuda.current_stream makes (3 us)
+_stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _run(x, fn, *args):
+    """fn(*args, current stream) on the device of the rows x."""
+    index = x.get_device()
+    if torch.cuda.current_device() == index:
+        _check(fn(*args, _stream_of(index)))
     else:
-        with torch.cuda.device(device):
-            _check(fn(args, torch.cuda.current_stream().cuda_stream))
+        with torch.cuda.device(index):
+            _check(fn(*args, _stream_of(index)))
 
 
 def _workspace(size, x):
-    return torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+    return x.new_empty(size, dtype=torch.uint8) if size else None
+
+
+def _new(x, shape, dtype=None):
+    """An uninitialised contiguous tensor beside x, in the current stream's memory."""
+    return x.new_empty(shape, dtype=dtype or x.dtype)
 
 
 def _differentiable(out, *tensors) -> bool:
@@ -236,9 +249,9 @@ def _conv_forward(x, weight, bias, frame_offsets, activation, initial_state, ret
     a.d_y, a.y_stride, a.zero_rest = y.data_ptr(), y.stride(0), out is None
     state = None
     if return_state:
-        state = torch.empty((n_seqs, width - 1, x.shape[1]), dtype=x.dtype, device=x.device)
+        state = _new(x, (n_seqs, width - 1, x.shape[1]))
         a.d_state = state.data_ptr()
-    _run(x.device, _lib.lib().mfcc_causal_conv, a)
+    _run(x, _lib.lib().mfcc_causal_conv, a)
     return y, state
 
 
@@ -282,15 +295,15 @@ def causal_conv_backward(dy, x, weight, bias=None, frame_offsets=None, *, activa
     dy = _rows(dy, "dy", x)
     channels = x.shape[1]
     dstate = _state(dstate, "dstate", (n_seqs, width - 1, channels), x.dtype, x)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    dweight = torch.empty((channels, width), dtype=torch.float32, device=x.device)
-    dbias = None if bias is None else torch.empty(channels, dtype=torch.float32, device=x.device)
-    dinitial = None if initial_state is None else torch.empty((n_seqs, width - 1, channels), dtype=x.dtype, device=x.device)
+    dx = _new(x, x.shape)
+    dweight = _new(x, (channels, width), torch.float32)
+    dbias = None if bias is None else _new(x, (channels,), torch.float32)
+    dinitial = None if initial_state is None else _new(x, (n_seqs, width - 1, channels))
     a.d_dy, a.dy_stride, a.d_dstate = dy.data_ptr(), dy.stride(0), _ptr(dstate)
     a.d_dx, a.dx_stride, a.d_dweight, a.d_dbias, a.d_dinitial = dx.data_ptr(), channels, dweight.data_ptr(), _ptr(dbias), _ptr(dinitial)
     ws = _workspace(_lib.lib().mfcc_causal_conv_backward_workspace(a), x)
     a.d_workspace, a.workspace_bytes = _ptr(ws), 0 if ws is None else ws.numel()
-    _run(x.device, _lib.lib().mfcc_causal_conv_backward, a)
+    _run(x, _lib.lib().mfcc_causal_conv_backward, a)
     return ConvGradients(dx, dweight, dbias, dinitial)
 
 
@@ -340,14 +353,9 @@ def causal_conv_step(x, state, weight, bias=None, *, activation=None, slots=None
     new_state = _next_state(state, _state(new_state, "new_state", (n_slots, width - 1, channels), x.dtype, x, writable=True))
     slots = _slots(slots, batch, x)
     y = _out(out, x, (x,))
-    lib = _lib.lib()
-
-    def call(_, stream):
-        return lib.mfcc_causal_conv_step(_DTYPE[x.dtype], batch, n_slots, channels, width, _ACTIVATION[activation],
-                                         x.data_ptr(), x.stride(0), state.data_ptr(), new_state.data_ptr(),
-                                         weight.data_ptr(), _ptr(bias), _ptr(slots), y.data_ptr(), y.stride(0), stream)
-
-    _run(x.device, call, None)
+    _run(x, _lib.lib().mfcc_causal_conv_step, _DTYPE[x.dtype], batch, n_slots, channels, width, _ACTIVATION[activation],
+         x.data_ptr(), x.stride(0), state.data_ptr(), new_state.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(slots),
+         y.data_ptr(), y.stride(0))
     return y
 
 
@@ -397,11 +405,11 @@ def _scan_forward(u, delta, A, B, Cm, D, delta_bias, frame_offsets, softplus, in
     a.d_y, a.y_stride, a.zero_rest = y.data_ptr(), y.stride(0), out is None
     final = None
     if return_state:
-        final = torch.empty(shape, dtype=torch.float32, device=u.device)
+        final = _new(u, shape, torch.float32)
         a.d_final = final.data_ptr()
     ws = _workspace(_lib.lib().mfcc_selective_scan_workspace(a), u)
     a.d_workspace, a.workspace_bytes = _ptr(ws), 0 if ws is None else ws.numel()
-    _run(u.device, _lib.lib().mfcc_selective_scan, a)
+    _run(u, _lib.lib().mfcc_selective_scan, a)
     return y, final
 
 
@@ -452,7 +460,7 @@ def selective_scan_backward(dy, u, delta, A, B, C, D=None, delta_bias=None, fram
     dstate = _state(dstate, "dstate", shape, torch.float32, u)
 
     def new(like, dtype):
-        return None if like is None else torch.empty(like.shape, dtype=dtype, device=u.device)
+        return None if like is None else _new(u, like.shape, dtype)
 
     f32 = torch.float32
     g = ScanGradients(new(u, u.dtype), new(u, u.dtype), new(A, f32), new(B, u.dtype), new(C, u.dtype), new(D, f32),
@@ -461,7 +469,7 @@ def selective_scan_backward(dy, u, delta, A, B, C, D=None, delta_bias=None, fram
     (a.d_du, a.d_ddelta, a.d_dA, a.d_dB, a.d_dC, a.d_dD, a.d_ddelta_bias, a.d_dinitial) = map(_ptr, g)
     ws = _workspace(_lib.lib().mfcc_selective_scan_backward_workspace(a), u)
     a.d_workspace, a.workspace_bytes = _ptr(ws), 0 if ws is None else ws.numel()
-    _run(u.device, _lib.lib().mfcc_selective_scan_backward, a)
+    _run(u, _lib.lib().mfcc_selective_scan_backward, a)
     return g
 
 
@@ -483,8 +491,7 @@ def selective_scan_step(u, delta, A, B, C, state, D=None, delta_bias=None, *, so
     y = _out(out, u, (u, delta, B.flatten(1), C.flatten(1)) if out is not None else ())
     a.d_initial, a.d_final = state.data_ptr(), new_state.data_ptr()
     a.d_y, a.y_stride = y.data_ptr(), y.stride(0)
-    lib = _lib.lib()
-    _run(u.device, lambda args, stream: lib.mfcc_selective_scan_step(args, n_slots, _ptr(slots), stream), a)
+    _run(u, _lib.lib().mfcc_selective_scan_step, a, n_slots, _ptr(slots))
     return y
 
 
@@ -526,13 +533,12 @@ def _add_norm_forward(x, residual, weight, bias, scale, norm, eps, residual_dtyp
     if residual is not None:
         residual = _rows(residual, "residual", x, rt)
     a, keep = _norm_args(x, weight, bias, scale, norm, eps, 1, False, rt)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    r = torch.empty(x.shape, dtype=rt, device=x.device)
+    y, r = _new(x, x.shape), _new(x, x.shape, rt)
     a.d_x, a.x_stride = x.data_ptr(), x.stride(0)
     if residual is not None:
         a.d_residual, a.residual_stride = residual.data_ptr(), residual.stride(0)
     a.d_y, a.y_stride, a.d_r, a.r_stride = y.data_ptr(), x.shape[1], r.data_ptr(), x.shape[1]
-    _run(x.device, _lib.lib().mfcc_add_norm, a)
+    _run(x, _lib.lib().mfcc_add_norm, a)
     return y, r
 
 
@@ -595,11 +601,11 @@ def add_norm_backward(dy, dr, r, weight=None, bias=None, *, x=None, scale=None, 
     channels = r.shape[1]
 
     def vector(like):
-        return None if like is None else torch.empty(channels, dtype=torch.float32, device=r.device)
+        return None if like is None else _new(r, (channels,), torch.float32)
 
-    dresidual = torch.empty(r.shape, dtype=r.dtype, device=r.device)
+    dresidual = _new(r, r.shape)
     one = r.dtype == dtype and not learned and a.scale_value == 1.0
-    dx = dresidual if one else torch.empty(r.shape, dtype=dtype, device=r.device)
+    dx = dresidual if one else _new(r, r.shape, dtype)
     g = AddNormGradients(dx, dresidual, vector(weight), vector(bias), vector(scale if learned else None))
     a.d_r, a.r_stride = r.data_ptr(), r.stride(0)
     if dy is not None:
@@ -614,7 +620,7 @@ def add_norm_backward(dy, dr, r, weight=None, bias=None, *, x=None, scale=None, 
     if g.weight is not None or g.bias is not None or g.scale is not None:
         ws = _workspace(_lib.lib().mfcc_norm_backward_workspace(a), r)
     a.d_workspace, a.workspace_bytes = _ptr(ws), 0 if ws is None else ws.numel()
-    _run(r.device, _lib.lib().mfcc_add_norm_backward, a)
+    _run(r, _lib.lib().mfcc_add_norm_backward, a)
     return g
 
 
@@ -640,7 +646,7 @@ def _gate_norm_forward(x, z, weight, bias, norm, groups, gate_first, eps, out):
     y = _out(out, x, (x, z))
     a.d_x, a.x_stride, a.d_z, a.z_stride = x.data_ptr(), x.stride(0), z.data_ptr(), z.stride(0)
     a.d_y, a.y_stride = y.data_ptr(), y.stride(0)
-    _run(x.device, _lib.lib().mfcc_gate_norm, a)
+    _run(x, _lib.lib().mfcc_gate_norm, a)
     return y
 
 
@@ -662,10 +668,9 @@ def gate_norm_backward(dy, x, z, weight=None, bias=None, *, norm="rms", groups=1
     channels = x.shape[1]
 
     def vector(like):
-        return None if like is None else torch.empty(channels, dtype=torch.float32, device=x.device)
+        return None if like is None else _new(x, (channels,), torch.float32)
 
-    g = GateNormGradients(torch.empty(x.shape, dtype=x.dtype, device=x.device),
-                          torch.empty(x.shape, dtype=x.dtype, device=x.device), vector(weight), vector(bias))
+    g = GateNormGradients(_new(x, x.shape), _new(x, x.shape), vector(weight), vector(bias))
     a.d_x, a.x_stride, a.d_z, a.z_stride = x.data_ptr(), x.stride(0), z.data_ptr(), z.stride(0)
     a.d_dy, a.dy_stride = dy.data_ptr(), dy.stride(0)
     a.d_dx, a.d_dz, a.d_dweight, a.d_dbias = g.x.data_ptr(), g.z.data_ptr(), _ptr(g.weight), _ptr(g.bias)
@@ -673,5 +678,5 @@ def gate_norm_backward(dy, x, z, weight=None, bias=None, *, norm="rms", groups=1
     if g.weight is not None or g.bias is not None:
         ws = _workspace(_lib.lib().mfcc_norm_backward_workspace(a), x)
     a.d_workspace, a.workspace_bytes = _ptr(ws), 0 if ws is None else ws.numel()
-    _run(x.device, _lib.lib().mfcc_gate_norm_backward, a)
+    _run(x, _lib.lib().mfcc_gate_norm_backward, a)
     return g
