@@ -9,6 +9,7 @@
 #include <cstring>
 #include <new>
 #include <string>
+#include <type_traits>
 
 #include "../../include/mfcc_hip.h"
 
@@ -43,29 +44,59 @@ struct F16 { using mem = _Float16; };
 template <typename M> __device__ __forceinline__ float widen(M v) { return (float)v; }
 template <typename M> __device__ __forceinline__ M narrow(float v) { return (M)v; }
 
-// VEC elements from an address that is only aligned to its element: global memory takes wide accesses
-// at any such address on gfx950, so a row of any width and stride uses the same 16-byte loads.
-// n < VEC (the ragged end of a row) goes element by element.
+// VEC elements as they lie in memory, in 32-bit words: in the 16-bit types half the registers until they are used,
+// and one wide access (an array of a 16-bit type takes a register, and often a load, per element: 166 instead of
+// 98 us for the convolution of 30011 x 4096).
+template <typename M, int VEC>
+struct Raw {
+    uint32_t u[VEC * sizeof(M) / 4];
+    __device__ __forceinline__ float get(int i) const {
+        if constexpr (sizeof(M) == 4) return __uint_as_float(u[i]);
+        else if constexpr (std::is_same<M, __bf16>::value) return __uint_as_float(i % 2 ? u[i / 2] & 0xffff0000u : u[i / 2] << 16);
+        else return (float)__builtin_bit_cast(M, (uint16_t)(u[i / 2] >> (i % 2 * 16)));
+    }
+    __device__ __forceinline__ void set(const float (&v)[VEC]) {
+        if constexpr (sizeof(M) == 4) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) u[i] = __float_as_uint(v[i]);
+        } else {
+            typedef float f2 __attribute__((ext_vector_type(2)));
+            typedef M m2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+            for (int i = 0; i < VEC; i += 2) u[i / 2] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){v[i], v[i + 1]}, m2));
+        }
+    }
+};
+
+// From and to an address that is only aligned to its element: global memory takes wide accesses at any such
+// address on gfx950, so a row of any width and stride uses the same loads.  n < VEC (the ragged end of a row) goes
+// element by element.
+template <typename M, int VEC>
+__device__ __forceinline__ void load_raw(Raw<M, VEC>& v, const M* __restrict__ p, int n) {
+    if (n >= VEC) {
+        __builtin_memcpy(v.u, p, sizeof(v.u));
+    } else {
+        float e[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) e[i] = i < n ? widen(p[i]) : 0.0f;
+        v.set(e);
+    }
+}
+
 template <typename M, int VEC>
 __device__ __forceinline__ void load_vec(float (&v)[VEC], const M* __restrict__ p, int n) {
-    if (n >= VEC) {
-        M raw[VEC];
-        __builtin_memcpy(raw, p, sizeof(raw));
+    Raw<M, VEC> raw;
+    load_raw<M, VEC>(raw, p, n);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) v[i] = widen(raw[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) v[i] = i < n ? widen(p[i]) : 0.0f;
-    }
+    for (int i = 0; i < VEC; ++i) v[i] = raw.get(i);
 }
 
 template <typename M, int VEC>
 __device__ __forceinline__ void store_vec(M* __restrict__ p, const float (&v)[VEC], int n) {
     if (n >= VEC) {
-        M raw[VEC];
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) raw[i] = narrow<M>(v[i]);
-        __builtin_memcpy(p, raw, sizeof(raw));
+        Raw<M, VEC> raw;
+        raw.set(v);
+        __builtin_memcpy(p, raw.u, sizeof(raw.u));
     } else {
 #pragma unroll
         for (int i = 0; i < VEC; ++i)
@@ -209,6 +240,13 @@ __device__ __forceinline__ SlotUse slot_use(const int32_t* __restrict__ slots, i
         after |= same && e > e0;
     }
     return {__ballot(before) != 0, __ballot(after) != 0};
+}
+
+// Workgroups are dealt to the eight XCDs in turn.  This gives each XCD a contiguous eighth of the work, so that
+// neighbouring pieces, which share rows, share an L2.
+__device__ __forceinline__ unsigned xcd_order(unsigned block, unsigned blocks) {
+    const unsigned each = blocks / 8, rest = blocks % 8, xcd = block % 8;
+    return xcd * each + min(xcd, rest) + block / 8;
 }
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }

@@ -11,7 +11,7 @@
 
 namespace packed {
 
-constexpr int GROUP = 4;      // rows per step of a thread
+constexpr int GROUP = 4;      // rows per step of a thread in the backward pass
 
 struct ConvFwd {
     const void* x; int64_t x_stride;
@@ -56,12 +56,15 @@ __device__ __forceinline__ void tap_of(float (&v)[VEC], const float (&near)[VEC]
     }
 }
 
-template <typename T, int K, int VEC>
+// A thread walks down its tile G rows at a time.  Waiting for memory is what bounds it, so the next G rows are in
+// flight while the current ones are computed, and rows are kept in their memory type (in float32 the window and
+// the rows ahead would cost half the wavefronts).
+template <typename T, int K, int VEC, int G>
 __global__ __launch_bounds__(256) void k_conv_fwd(const ConvFwd a) {
     using M = typename T::mem;
-    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t r0 = id / a.n_vec * a.tile;
-    const int c0 = (int)(id % a.n_vec) * VEC;
+    const unsigned id = xcd_order(blockIdx.x, gridDim.x) * 256 + threadIdx.x;      // below 2^31
+    const int64_t r0 = (int64_t)(id / (unsigned)a.n_vec) * a.tile;
+    const int c0 = (int)(id % (unsigned)a.n_vec) * VEC;
     if (r0 >= a.rows) return;
     const int n = a.channels - c0;
     const int64_t r1 = min(r0 + a.tile, a.rows);
@@ -69,59 +72,71 @@ __global__ __launch_bounds__(256) void k_conv_fwd(const ConvFwd a) {
     M* y = static_cast<M*>(a.y) + c0;
     const M* initial = static_cast<const M*>(a.initial);
 
+    Raw<M, VEC> line[K - 1 + G], next[G];
+    auto fetch = [&](int64_t r) {
+#pragma unroll
+        for (int g = 0; g < G; ++g) load_raw<M, VEC>(next[g], x + min(r + g, r1 - 1) * a.x_stride, n);
+    };
+    fetch(r0);
+#pragma unroll
+    for (int j = 0; j < K - 1; ++j) load_raw<M, VEC>(line[j], x + max(r0 - (K - 1) + j, (int64_t)0) * a.x_stride, n);
     float w[K][VEC], b[VEC];
     load_taps<K, VEC>(w, b, a.w, a.bias, c0, n);
-    float win[K - 1 + GROUP][VEC];         // the K - 1 rows before the group, then the group
-#pragma unroll
-    for (int j = 0; j < K - 1; ++j)
-        load_vec<M, VEC>(win[j], x + max(r0 - (K - 1) + j, (int64_t)0) * a.x_stride, n);
-
     Place q = find_row(a.off, a.n_seqs, a.rows, r0);
-    for (int64_t r = r0; r < r1; r += GROUP) {
+    auto finish = [&](float (&acc)[VEC], int64_t row) {
+        if (a.act) {
 #pragma unroll
-        for (int g = 0; g < GROUP; ++g) load_vec<M, VEC>(win[K - 1 + g], x + min(r + g, a.rows - 1) * a.x_stride, n);
-        const bool plain = q.inside && r >= q.start + (K - 1) && r + GROUP <= min(q.end, r1);
+            for (int i = 0; i < VEC; ++i) acc[i] *= sigmoid_f<sizeof(M) == 4>(acc[i]);
+        }
+        store_vec<M, VEC>(y + row * a.y_stride, acc, n);
+    };
+    for (int64_t r = r0; r < r1; r += G) {
 #pragma unroll
-        for (int g = 0; g < GROUP; ++g) {
-            const int64_t row = r + g;
-            if (!plain) {
+        for (int g = 0; g < G; ++g) line[K - 1 + g] = next[g];
+        if (r + G < r1) fetch(r + G);
+        if (q.inside && r >= q.start + (K - 1) && r + G <= min(q.end, r1)) {
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                float acc[VEC];
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    acc[i] = b[i];
+#pragma unroll
+                    for (int j = 0; j < K; ++j) acc[i] = fmaf(w[j][i], line[g + j].get(i), acc[i]);
+                }
+                finish(acc, r + g);
+            }
+        } else {
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const int64_t row = r + g;
                 if (row >= r1) break;
                 if (row >= q.until) q = find_row(a.off, a.n_seqs, a.rows, row);
-            }
-            float acc[VEC];
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) acc[i] = b[i];
-            if (plain) {
-#pragma unroll
-                for (int j = 0; j < K; ++j)
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) acc[i] = fmaf(w[j][i], win[g + j][i], acc[i]);
-            } else {
+                float acc[VEC];
                 if (!q.inside) {
                     if (a.zero_rest) {
-                        float z[VEC] = {};
-                        store_vec<M, VEC>(y + row * a.y_stride, z, n);
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i) acc[i] = 0.0f;
+                        store_vec<M, VEC>(y + row * a.y_stride, acc, n);
                     }
                     continue;
                 }
 #pragma unroll
+                for (int i = 0; i < VEC; ++i) acc[i] = b[i];
+#pragma unroll
                 for (int j = 0; j < K; ++j) {
-                    float v[VEC];
-                    tap_of<M, K, VEC>(v, win[g + j], initial, q, row, K - 1 - j, a.channels, c0, n);
+                    float v[VEC], near[VEC];
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) near[i] = line[g + j].get(i);
+                    tap_of<M, K, VEC>(v, near, initial, q, row, K - 1 - j, a.channels, c0, n);
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) acc[i] = fmaf(w[j][i], v[i], acc[i]);
                 }
+                finish(acc, row);
             }
-            if (a.act) {
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) acc[i] *= sigmoid_f(acc[i]);
-            }
-            store_vec<M, VEC>(y + row * a.y_stride, acc, n);
         }
 #pragma unroll
-        for (int j = 0; j < K - 1; ++j)
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) win[j][i] = win[j + GROUP][i];
+        for (int j = 0; j < K - 1; ++j) line[j] = line[j + G];
     }
 }
 
@@ -228,7 +243,7 @@ __global__ __launch_bounds__(256) void k_conv_bwd(const ConvBwd a) {
                             float p = b[i];
 #pragma unroll
                             for (int j = 0; j < K; ++j) p = fmaf(w[j][i], tap[j][i], p);
-                            const float sg = sigmoid_f(p);
+                            const float sg = sigmoid_f<sizeof(M) == 4>(p);
                             d[i] *= sg * fmaf(p, 1.0f - sg, 1.0f);
                         }
                     }
@@ -434,17 +449,17 @@ __global__ __launch_bounds__(256) void k_conv_step(const ConvStep a) {
     for (int j = 0; j < K - 1; ++j) store_vec<M, VEC>(next + (int64_t)j * a.channels, win[j], n);
 }
 
-// Channels of a thread: 16 bytes of them forward; four in the backward pass, whose taps, sums and two
-// windows would otherwise leave one wavefront per SIMD.
-template <typename T> constexpr int conv_vec() { return 16 / (int)sizeof(typename T::mem); }
-constexpr int CONV_BWD_VEC = 4;
+// Channels of a thread: four in every type.  With the eight that make 16 bytes in the 16-bit types the taps, sums
+// and rows in flight cost half the wavefronts (125 against 98 us for 30011 x 4096).
+constexpr int CONV_VEC = 4;
+constexpr int CONV_AHEAD = 8;      // rows in flight of the forward pass
 
-// Rows per thread of the forward pass: long tiles read the K - 1 rows of overlap less often, but below
-// about four wavefronts per SIMD (256 CUs x 4) the chip is not full.
+// Rows per thread of the forward pass: a long tile reads its taps and the K - 1 rows of overlap less often, but
+// below about eight wavefronts per SIMD (256 CUs x 4) the chip is not full.
 inline int conv_fwd_tile(int64_t rows, int n_vec) {
-    for (int tile : {32, 16, 8})
-        if (ceil_div(rows, tile) * n_vec >= 4 * 1024 * WAVE) return tile;
-    return GROUP;
+    for (int tile : {128, 64, 32, 16})
+        if (ceil_div(rows, tile) * n_vec >= 8 * 1024 * WAVE) return tile;
+    return 8;
 }
 
 // Rows per wavefront of the backward pass (it also writes K + 1 partial sums per four tiles).
@@ -455,7 +470,7 @@ inline int conv_bwd_tile(int64_t rows, int n_vec) {
 }
 
 inline int64_t conv_bwd_parts(const mfcc_conv_args* a) {
-    return ceil_div(a->rows, 4 * (int64_t)conv_bwd_tile(a->rows, (int)ceil_div(a->channels, CONV_BWD_VEC)));
+    return ceil_div(a->rows, 4 * (int64_t)conv_bwd_tile(a->rows, (int)ceil_div(a->channels, CONV_VEC)));
 }
 
 template <typename Fn>
@@ -477,7 +492,7 @@ int by_width(int width, Fn&& fn) {
 template <typename T>
 int conv_forward(const mfcc_conv_args* a, hipStream_t st) {
     using M = typename T::mem;
-    constexpr int VEC = conv_vec<T>();
+    constexpr int VEC = CONV_VEC;
     return by_width(a->width, [&](auto width) {
         constexpr int K = decltype(width)::value;
         if (a->rows > 0) {
@@ -488,7 +503,7 @@ int conv_forward(const mfcc_conv_args* a, hipStream_t st) {
             f.tile = conv_fwd_tile(a->rows, f.n_vec); f.zero_rest = a->zero_rest; f.act = a->activation == MFCC_ACT_SILU;
             const int64_t blocks = ceil_div(ceil_div(a->rows, f.tile) * f.n_vec, 256);
             if (blocks > 0x7fffff) return mfcc_detail::fail(MFCC_E_UNSUPPORTED, "batch too large: split it");
-            hipLaunchKernelGGL((k_conv_fwd<T, K, VEC>), dim3((unsigned)blocks), dim3(256), 0, st, f);
+            hipLaunchKernelGGL((k_conv_fwd<T, K, VEC, CONV_AHEAD>), dim3((unsigned)blocks), dim3(256), 0, st, f);
             PACKED_LAUNCHED();
         }
         if (a->d_state && a->n_seqs > 0 && K > 1) {
@@ -512,11 +527,11 @@ int conv_backward(const mfcc_conv_args* a, hipStream_t st) {
         f.bias = a->d_bias; f.off = a->d_offsets; f.initial = a->d_initial; f.dstate = a->d_dstate; f.dx = a->d_dx;
         f.dx_stride = a->dx_stride; f.part = static_cast<float*>(a->d_workspace); f.dinitial = a->d_dinitial;
         f.rows = a->rows; f.n_seqs = a->n_seqs; f.channels = a->channels; f.act = a->activation == MFCC_ACT_SILU;
-        f.n_vec = (int)ceil_div(a->channels, CONV_BWD_VEC); f.tile = conv_bwd_tile(a->rows, f.n_vec);
+        f.n_vec = (int)ceil_div(a->channels, CONV_VEC); f.tile = conv_bwd_tile(a->rows, f.n_vec);
         const int64_t parts = conv_bwd_parts(a);
         if (parts > 65535) return mfcc_detail::fail(MFCC_E_UNSUPPORTED, "batch too large: split it");
         if (a->rows > 0) {
-            hipLaunchKernelGGL((k_conv_bwd<T, K, CONV_BWD_VEC>), dim3((unsigned)ceil_div(f.n_vec, WAVE), (unsigned)parts),
+            hipLaunchKernelGGL((k_conv_bwd<T, K, CONV_VEC>), dim3((unsigned)ceil_div(f.n_vec, WAVE), (unsigned)parts),
                                dim3(256), 0, st, f);
             PACKED_LAUNCHED();
         }
@@ -534,7 +549,7 @@ int conv_backward(const mfcc_conv_args* a, hipStream_t st) {
 
 template <typename T>
 int conv_step(ConvStep f, int width, hipStream_t st) {
-    constexpr int VEC = conv_vec<T>();
+    constexpr int VEC = CONV_VEC;
     return by_width(width, [&](auto w) {
         constexpr int K = decltype(w)::value;
         f.n_vec = (int)ceil_div(f.channels, VEC);

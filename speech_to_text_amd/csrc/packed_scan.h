@@ -444,8 +444,8 @@ __device__ __forceinline__ float sum_channels(float v) {     // over the lanes o
     return v;
 }
 
-// Eight neighbouring elements in LDS, 16 bytes aligned; left in their type (the registers) until they are used.
-template <typename M> struct alignas(16) Eight { M e[SUB]; };
+// Eight neighbouring elements in LDS, 16 bytes aligned.
+template <typename M> struct alignas(16) Eight { Raw<M, SUB> r; };
 
 template <typename T, int NP>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(bwd_waves<T, NP>()))) void k_scan_bwd(const Scan a) {
@@ -575,7 +575,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(bwd_waves<T
             }
             float b[4];
             four(b, pB + j * NP);
-            const float d = d8.e[j], du = d * widen(u8.e[j]);
+            const float d = d8.r.get(j), du = d * u8.r.get(j);
 #pragma unroll
             for (int i = 0; i < 4; ++i) h[i] = fmaf(exp2_hw(d * A2[i]), h[i], du * b[i]);
         }
@@ -595,8 +595,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(bwd_waves<T
     auto back = [&](auto plain, int s) {
         constexpr bool PLAIN = decltype(plain)::value;
         float hs[SUB + 1][4], ea[SUB][4];
-        Eight<float> d8 = *reinterpret_cast<const Eight<float>*>(pd + s * SUB);      // d, then its gradient
-        Eight<M> u8 = *reinterpret_cast<const Eight<M>*>(pu + s * SUB);              // u, then its gradient
+        float dd[SUB] = {}, gu[SUB] = {};
+        const Eight<float> d8 = *reinterpret_cast<const Eight<float>*>(pd + s * SUB);
+        const Eight<M> u8 = *reinterpret_cast<const Eight<M>*>(pu + s * SUB);
         const Eight<M> y8 = *reinterpret_cast<const Eight<M>*>(pdy + s * SUB);
         int at = s * SUB * NP + n0;                      // of the lane's four B in the row, and C
 #pragma unroll
@@ -617,7 +618,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(bwd_waves<T
                 if (flag & START) enter(prev, t, flag, a.initial);
             }
             four(b, sB + at + j * NP);
-            const float d = d8.e[j], du = d * widen(u8.e[j]);
+            const float d = d8.r.get(j), du = d * u8.r.get(j);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 ea[j][i] = exp2_hw(d * A2[i]);
@@ -640,7 +641,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(bwd_waves<T
             }
             four(b, sB + at + j * NP);
             four(cc, sC + at + j * NP);
-            const float d = d8.e[j], uv = widen(u8.e[j]), dv = widen(y8.e[j]), du = d * uv;
+            const float d = d8.r.get(j), uv = u8.r.get(j), dv = y8.r.get(j), du = d * uv;
             float gB = 0.0f, wA = 0.0f;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -658,8 +659,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(bwd_waves<T
                 store_vec<float, 4>(a.dinitial + ((int64_t)sseq[t] * a.channels + c) * a.state + n0, G, n_left);
             gB = sum_states<LPC>(gB);
             wA = sum_states<LPC>(wA);
-            d8.e[j] = fmaf(uv, gB, wA * LN2);              // A = A2 ln 2
-            u8.e[j] = narrow<M>(fmaf(d, gB, skip * dv));
+            dd[j] = fmaf(uv, gB, wA * LN2);                // A = A2 ln 2
+            gu[j] = fmaf(d, gB, skip * dv);
             const float w0 = halve32(red[0], red[4]), w1 = halve32(red[1], red[5]);
             const float w2 = halve32(red[2], red[6]), w3 = halve32(red[3], red[7]);
             const float v0 = sum_channels<LPC>(halve16(w0, w2)), v1 = sum_channels<LPC>(halve16(w1, w3));
@@ -667,8 +668,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(bwd_waves<T
             *reinterpret_cast<float2*>(pslab + (s & 1) * SLAB + j * 2 * NP) = make_float2(v0, v1);
         }
         if (nq == 0) {
-            *reinterpret_cast<Eight<float>*>(pd + s * SUB) = d8;
-            *reinterpret_cast<Eight<M>*>(pu + s * SUB) = u8;
+            Eight<float> d_out;
+            Eight<M> u_out;
+            d_out.r.set(dd);
+            u_out.r.set(gu);
+            *reinterpret_cast<Eight<float>*>(pd + s * SUB) = d_out;
+            *reinterpret_cast<Eight<M>*>(pu + s * SUB) = u_out;
         }
     };
     float* const part_bc = a.part_bc + ((int64_t)gb * a.rows + r0) * a.groups * NP + (int64_t)g * NP;
