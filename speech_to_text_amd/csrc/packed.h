@@ -251,6 +251,21 @@ __device__ __forceinline__ unsigned xcd_order(unsigned block, unsigned blocks) {
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// p[first] + p[first + step] + ... of `count` terms `stride` apart, eight loads in flight; a fixed order.
+__device__ __forceinline__ float sum_strided(const float* __restrict__ p, int64_t first, int64_t step, int64_t count,
+                                             int64_t stride) {
+    float s = 0.0f;
+    int64_t i = first;
+    for (; i + 7 * step < count; i += 8 * step) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = p[(i + j * step) * stride];
+        s += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+    }
+    for (; i < count; i += step) s += p[i * stride];
+    return s;
+}
+
 template <typename Fn>
 int by_type(int dtype, Fn&& fn) {
     switch (dtype) {

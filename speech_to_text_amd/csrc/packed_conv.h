@@ -198,22 +198,28 @@ __global__ __launch_bounds__(256) void k_conv_bwd(const ConvBwd a) {
     if (live && r0 < a.rows) {
         float w[K][VEC], b[VEC];
         load_taps<K, VEC>(w, b, a.w, a.bias, c0, n);
-        float win[K - 1 + GROUP][VEC], dp[K - 1 + GROUP][VEC];
+        Raw<M, VEC> line[K - 1 + GROUP], dyr[GROUP], next_x[GROUP], next_dy[GROUP];
+        float dp[K - 1 + GROUP][VEC];
+        auto fetch = [&](int64_t r) {
+#pragma unroll
+            for (int g = 0; g < GROUP; ++g) {
+                const int64_t row = min(r + g, a.rows - 1);
+                load_raw<M, VEC>(next_x[g], x + row * a.x_stride, n);
+                load_raw<M, VEC>(next_dy[g], dy + row * a.dy_stride, n);
+            }
+        };
+        fetch(r0);
 #pragma unroll
         for (int j = 0; j < K - 1; ++j) {
-            load_vec<M, VEC>(win[j], x + max(r0 - (K - 1) + j, (int64_t)0) * a.x_stride, n);
+            load_raw<M, VEC>(line[j], x + max(r0 - (K - 1) + j, (int64_t)0) * a.x_stride, n);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) dp[j][i] = 0.0f;    // rows before the tile: their dx belongs to the tile above
         }
         Place q = find_row(a.off, a.n_seqs, a.rows, r0);
         for (int64_t r = r0; r < r1 + (K - 1); r += GROUP) {
-            float dyv[GROUP][VEC];
 #pragma unroll
-            for (int g = 0; g < GROUP; ++g) {
-                const int64_t row = min(r + g, a.rows - 1);
-                load_vec<M, VEC>(win[K - 1 + g], x + row * a.x_stride, n);
-                load_vec<M, VEC>(dyv[g], dy + row * a.dy_stride, n);
-            }
+            for (int g = 0; g < GROUP; ++g) { line[K - 1 + g] = next_x[g]; dyr[g] = next_dy[g]; }
+            if (r + GROUP < r1 + (K - 1)) fetch(r + GROUP);
             // the whole group, and the rows whose dx it completes, inside one sequence and this tile
             const bool plain = q.inside && r - (K - 1) >= q.start && r - (K - 1) >= r0 && r + GROUP <= min(q.end, r1);
 #pragma unroll
@@ -229,16 +235,14 @@ __global__ __launch_bounds__(256) void k_conv_bwd(const ConvBwd a) {
                     float tap[K][VEC];
 #pragma unroll
                     for (int j = 0; j < K; ++j) {
-                        if (plain) {
+                        float near[VEC];
 #pragma unroll
-                            for (int i = 0; i < VEC; ++i) tap[j][i] = win[g + j][i];
-                        } else {
-                            tap_of<M, K, VEC>(tap[j], win[g + j], initial, q, row, K - 1 - j, a.channels, c0, n);
-                        }
+                        for (int i = 0; i < VEC; ++i) tap[j][i] = near[i] = line[g + j].get(i);
+                        if (!plain) tap_of<M, K, VEC>(tap[j], near, initial, q, row, K - 1 - j, a.channels, c0, n);
                     }
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) {
-                        d[i] = dyv[g][i];
+                        d[i] = dyr[g].get(i);
                         if (a.act) {
                             float p = b[i];
 #pragma unroll
@@ -291,11 +295,11 @@ __global__ __launch_bounds__(256) void k_conv_bwd(const ConvBwd a) {
             }
 #pragma unroll
             for (int j = 0; j < K - 1; ++j)
+{
+                line[j] = line[j + GROUP];
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    win[j][i] = win[j + GROUP][i];
-                    dp[j][i] = dp[j + GROUP][i];
-                }
+                for (int i = 0; i < VEC; ++i) dp[j][i] = dp[j + GROUP][i];
+            }
         }
     }
     // the four row tiles of the block, then one partial sum per block: a fixed order, the same on every run
@@ -318,19 +322,18 @@ __global__ __launch_bounds__(256) void k_conv_bwd(const ConvBwd a) {
 
 // dweight (channels, K) and dbias (channels) from the partial sums.
 template <typename T>
-__global__ __launch_bounds__(256) void k_conv_sum(const float* __restrict__ part, int64_t n_part, int K, int channels,
-                                                  float* __restrict__ dweight, float* __restrict__ dbias) {
-    __shared__ float sh[4][64];
+__global__ __launch_bounds__(1024) void k_conv_sum(const float* __restrict__ part, int64_t n_part, int K, int channels,
+                                                   float* __restrict__ dweight, float* __restrict__ dbias) {
+    __shared__ float sh[16][64];
     const int lane = threadIdx.x & 63, slice = threadIdx.x >> 6;
     const int64_t m = (int64_t)(K + 1) * channels;
     const int64_t e = (int64_t)blockIdx.x * 64 + lane;
-    float s = 0.0f;
-    if (e < m)
-        for (int64_t p = slice; p < n_part; p += 4) s += part[p * m + e];
-    sh[slice][lane] = s;
+    sh[slice][lane] = e < m ? sum_strided(part + e, slice, 16, n_part, m) : 0.0f;
     __syncthreads();
     if (slice == 0 && e < m) {
-        const float v = (sh[0][lane] + sh[1][lane]) + (sh[2][lane] + sh[3][lane]);
+        float v = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v += sh[i][lane];
         const int j = (int)(e / channels), c = (int)(e % channels);
         if (j < K) dweight[(int64_t)c * K + j] = v;
         else if (dbias) dbias[c] = v;
@@ -535,7 +538,7 @@ int conv_backward(const mfcc_conv_args* a, hipStream_t st) {
                                dim3(256), 0, st, f);
             PACKED_LAUNCHED();
         }
-        hipLaunchKernelGGL(k_conv_sum<T>, dim3((unsigned)ceil_div((int64_t)(K + 1) * a->channels, 64)), dim3(256), 0, st,
+        hipLaunchKernelGGL(k_conv_sum<T>, dim3((unsigned)ceil_div((int64_t)(K + 1) * a->channels, 64)), dim3(1024), 0, st,
                            f.part, parts, K, a->channels, a->d_dweight, a->d_dbias);
         PACKED_LAUNCHED();
         if (a->d_dinitial && a->n_seqs > 0 && K > 1) {

@@ -269,10 +269,7 @@ __global__ __launch_bounds__(1024) void k_norm_reduce(const float* __restrict__ 
     const int c = blockIdx.x * 64 + lane, j = blockIdx.y;
     float* out = j == 0 ? dweight : j == 1 ? dbias : dscale;
     if (!out) return;
-    float s = 0.0f;
-    if (c < channels)
-        for (int p = slice; p < n_part; p += 16) s += part[((int64_t)p * 3 + j) * channels + c];
-    sh[slice][lane] = s;
+    sh[slice][lane] = c < channels ? sum_strided(part + (int64_t)j * channels + c, slice, 16, n_part, 3 * (int64_t)channels) : 0.0f;
     __syncthreads();
     if (slice == 0 && c < channels) {
         float t = 0.0f;

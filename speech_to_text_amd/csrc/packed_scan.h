@@ -749,15 +749,7 @@ __global__ __launch_bounds__(1024) void k_scan_reduce(const ReduceJobs jobs) {
     // few parts: the slices take different elements instead
     const bool few = job.n_part < 64;
     const int64_t e = ((int64_t)blockIdx.x - job.first_block) * (few ? 1024 : 64) + (few ? threadIdx.x : lane);
-    float s = 0.0f;
-    if (e < job.m) {
-        const float* p = job.part + e;
-        const int step = few ? 1 : 16;
-        int64_t i = few ? 0 : slice;
-        for (; i + 3 * step < job.n_part; i += 4 * step)
-            s += (p[i * job.m] + p[(i + step) * job.m]) + (p[(i + 2 * step) * job.m] + p[(i + 3 * step) * job.m]);
-        for (; i < job.n_part; i += step) s += p[i * job.m];
-    }
+    float s = e < job.m ? sum_strided(job.part + e, few ? 0 : slice, few ? 1 : 16, job.n_part, job.m) : 0.0f;
     if (!few) {
         sh[slice][lane] = s;
         __syncthreads();
