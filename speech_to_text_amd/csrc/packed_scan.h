@@ -44,6 +44,24 @@ __device__ __forceinline__ float step_of(int softplus, M raw, float bias) {
     const float v = widen(raw) + bias;
     return softplus ? softplus_f<sizeof(M) == 4>(v) : v;
 }
+template <int COUNT, typename M>
+__device__ __forceinline__ void steps_of(float (&d)[COUNT], int softplus, const M (&raw)[COUNT], float bias) {
+    if (softplus) {                     // the branch outside: what a block knows of its values saves operations
+#pragma unroll
+        for (int j = 0; j < COUNT; ++j) d[j] = softplus_f<sizeof(M) == 4>(widen(raw[j]) + bias);
+    } else {
+#pragma unroll
+        for (int j = 0; j < COUNT; ++j) d[j] = widen(raw[j]) + bias;
+    }
+}
+
+// base[c] with the row in scalar registers and the lane's share as a 32-bit byte offset: one memory instruction
+// without address arithmetic.
+template <typename M>
+__device__ __forceinline__ M& lane_at(M* base, unsigned lane_bytes) {
+    using Byte = std::conditional_t<std::is_const<M>::value, const char, char>;
+    return *reinterpret_cast<M*>(reinterpret_cast<Byte*>(base) + lane_bytes);
+}
 
 // The next rows of a wavefront's channels, loaded while the ones before them are worked on.  The row is in
 // scalar registers, the lane adds its channel.
@@ -51,16 +69,17 @@ constexpr int AHEAD = 4;
 template <typename M, bool BACK>
 struct Ahead {
     M u[AHEAD], delta[AHEAD], dy[BACK ? AHEAD : 1];
-    // rows t .. t + 3 of the chunk at r0, its last one instead of those behind it
-    __device__ __forceinline__ void load(const Scan& a, int64_t r0, int t, int len, unsigned c) {
+    // rows t .. t + 3 of the chunk at r0, its last one instead of those behind it, at the lane's byte offset
+    __device__ __forceinline__ void load(const Scan& a, int64_t r0, int t, int len, unsigned at) {
+        asm volatile("" : "+v"(at));       // hoisted out of the loop, the offset becomes 64 bits wide and is added by the lanes
         const M* pu = static_cast<const M*>(a.u) + (r0 + t) * a.u_stride;
         const M* pd = static_cast<const M*>(a.delta) + (r0 + t) * a.delta_stride;
         const M* py = BACK ? static_cast<const M*>(a.dy) + (r0 + t) * a.dy_stride : nullptr;
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) {
-            u[j] = pu[c];
-            delta[j] = pd[c];
-            if (BACK) dy[j] = py[c];
+            u[j] = lane_at(pu, at);
+            delta[j] = lane_at(pd, at);
+            if (BACK) dy[j] = lane_at(py, at);
             if (t + j + 1 < len) {
                 pu += a.u_stride;
                 pd += a.delta_stride;
@@ -87,6 +106,7 @@ __device__ __forceinline__ void row_of(float (&v)[SIZE], const float* p) {
     }
 }
 
+// `state` columns from src on, padded with zeros.
 template <typename M, int NP>
 __device__ __forceinline__ void stage_rows(float* lds, const M* __restrict__ src, int64_t stride, int64_t row, int count,
                                            int state) {
@@ -96,16 +116,16 @@ __device__ __forceinline__ void stage_rows(float* lds, const M* __restrict__ src
     }
 }
 
-// A channel's states in an (sequence, channel, n) array; zeros without the array.  Rarely run inside the loop
-// over rows: the opaque offset and count keep the compiler from holding its sixteen addresses and lane masks in
+// A channel's states from n0 on in an (sequence, channel, n) array; zeros without the array.  Rarely run inside the
+// loop over rows: the opaque offset and count keep the compiler from holding its sixteen addresses and lane masks in
 // registers throughout.
 template <int NP>
-__device__ __forceinline__ void load_state(float (&v)[NP], const float* from, const Scan& a, int s, int c) {
+__device__ __forceinline__ void load_state(float (&v)[NP], const float* from, const Scan& a, int s, int c, int n0) {
 #pragma unroll
     for (int n = 0; n < NP; ++n) v[n] = 0.0f;
     if (!from) return;
-    int64_t at = ((int64_t)s * a.channels + c) * a.state;
-    int count = a.state;
+    int64_t at = ((int64_t)s * a.channels + c) * a.state + n0;
+    int count = a.state - n0;
     asm volatile("" : "+v"(at), "+s"(count));
 #pragma unroll
     for (int n = 0; n < NP; ++n) {
@@ -124,43 +144,46 @@ __device__ __forceinline__ void store_state(float* to, const float (&v)[NP], con
 }
 
 template <int NP>
-__device__ __forceinline__ void load_rates(float (&A2)[NP], const Scan& a, int c) {
+__device__ __forceinline__ void load_rates(float (&A2)[NP], const Scan& a, int c, int n0) {
 #pragma unroll
-    for (int n = 0; n < NP; ++n) A2[n] = n < a.state ? a.A[(int64_t)c * a.state + n] * SCAN_LOG2E : 0.0f;
+    for (int n = 0; n < NP; ++n) A2[n] = n0 + n < a.state ? a.A[(int64_t)c * a.state + n0 + n] * SCAN_LOG2E : 0.0f;
 }
 
-// Pass 1.  A lane holds a channel and all its states; B and C come from LDS.
+// Pass 1.  A lane holds a channel and up to sixteen of its states (they are independent here: more of them are
+// more workgroups); B and C come from LDS.
 template <typename T, int NP, bool BACK>
 __global__ __launch_bounds__(256) void k_scan_sum(const Scan a) {
     using M = typename T::mem;
     __shared__ float sB[SCAN_TILE * NP], sC[BACK ? SCAN_TILE * NP : 1];
-    const int n_blocks = a.groups * a.blocks_per_group;
-    const int cb = blockIdx.x % n_blocks, k = blockIdx.x / n_blocks;
+    const int slices = (a.state + NP - 1) / NP, n_blocks = a.groups * a.blocks_per_group * slices;
+    const int sb = blockIdx.x % n_blocks, k = blockIdx.x / n_blocks;
+    const int cb = sb / slices, n0 = sb % slices * NP;
     const int g = cb / a.blocks_per_group;
     const int in_group = (cb % a.blocks_per_group) * blockDim.x + threadIdx.x;
     const bool live = in_group < a.per;
     const int c = g * a.per + (live ? in_group : 0);
     const int64_t r0 = (int64_t)k * a.chunk;
     const int len = (int)min((int64_t)a.chunk, a.rows - r0);
-    const M* B = static_cast<const M*>(a.B) + (int64_t)g * a.state;
-    const M* C = static_cast<const M*>(a.C) + (int64_t)g * a.state;
+    const M* B = static_cast<const M*>(a.B) + (int64_t)g * a.state + n0;
+    const M* C = static_cast<const M*>(a.C) + (int64_t)g * a.state + n0;
     const float bias = a.bias ? a.bias[c] : 0.0f;
 
     float A2[NP], h[NP], P[NP], R[NP];
-    load_rates<NP>(A2, a, c);
+    load_rates<NP>(A2, a, c, n0);
 #pragma unroll
     for (int n = 0; n < NP; ++n) { h[n] = 0.0f; P[n] = 1.0f; R[n] = 0.0f; }
     float sum = 0.0f;
     int reset = 0;                 // a sequence start was passed: the reverse part is complete
 
     Ahead<M, BACK> next;
-    next.load(a, r0, 0, len, c);
+    unsigned lane_bytes = (unsigned)c * sizeof(M);       // below 2^26 (2^24 channels)
+    next.load(a, r0, 0, len, lane_bytes);
     Stretch q = find_stretch(a.off, a.n_seqs, a.rows, r0, 0, len);
     for (int t0 = 0; t0 < len; t0 += SCAN_TILE) {
         const int t1 = min(t0 + SCAN_TILE, len);
         __syncthreads();
-        stage_rows<M, NP>(sB, B, a.B_stride, r0 + t0, t1 - t0, a.state);
-        if (BACK) stage_rows<M, NP>(sC, C, a.C_stride, r0 + t0, t1 - t0, a.state);
+        stage_rows<M, NP>(sB, B, a.B_stride, r0 + t0, t1 - t0, a.state - n0);
+        if (BACK) stage_rows<M, NP>(sC, C, a.C_stride, r0 + t0, t1 - t0, a.state - n0);
         __syncthreads();
         for (int t = t0; t < t1;) {
             if (t >= q.until) q = find_stretch(a.off, a.n_seqs, a.rows, r0, t, len);
@@ -168,12 +191,12 @@ __global__ __launch_bounds__(256) void k_scan_sum(const Scan a) {
             if (!q.inside || q.first) {
                 reset = uniform(1);
                 sum = 0.0f;
-                load_state<NP>(h, q.inside ? a.initial : nullptr, a, q.s, c);
+                load_state<NP>(h, q.inside ? a.initial : nullptr, a, q.s, c, n0);
                 q.first = false;
             }
             if (!q.inside) {
                 t = t2;
-                if (t < len) next.load(a, r0, t, len, c);
+                if (t < len) next.load(a, r0, t, len, lane_bytes);
                 continue;
             }
             // rows t .. t2 in groups of four; OPEN: the reverse part still runs
@@ -183,11 +206,11 @@ __global__ __launch_bounds__(256) void k_scan_sum(const Scan a) {
                     const int from = t, count = uniform(min(AHEAD, t2 - t));
                     const Ahead<M, BACK> now = next;
                     t = uniform(t + count);
-                    if (t < len) next.load(a, r0, t, len, c);
+                    if (t < len) next.load(a, r0, t, len, lane_bytes);
                     float d[AHEAD], du[AHEAD], dv[AHEAD];
+                    steps_of<AHEAD>(d, a.softplus, now.delta, bias);
 #pragma unroll
                     for (int j = 0; j < AHEAD; ++j) {
-                        d[j] = step_of(a.softplus, now.delta[j], bias);
                         du[j] = d[j] * widen(now.u[j]);
                         dv[j] = OPEN ? widen(now.dy[j]) : 0.0f;
                     }
@@ -221,7 +244,7 @@ __global__ __launch_bounds__(256) void k_scan_sum(const Scan a) {
             else advance(std::false_type{});
             if (BACK && a.dfinal && !reset && q.last && t == q.until) {   // the gradient of the state left behind enters here
                 float g_end[NP];
-                load_state<NP>(g_end, a.dfinal, a, q.s, c);
+                load_state<NP>(g_end, a.dfinal, a, q.s, c, n0);
 #pragma unroll
                 for (int n = 0; n < NP; ++n) R[n] = fmaf(P[n], g_end[n], R[n]);
             }
@@ -230,18 +253,19 @@ __global__ __launch_bounds__(256) void k_scan_sum(const Scan a) {
     if (!live) return;
 #pragma unroll
     for (int n = 0; n < NP; ++n)
-        if (n < a.state) {
-            const int64_t at = ((int64_t)k * a.state + n) * a.channels + c;
+        if (n0 + n < a.state) {
+            const int64_t at = ((int64_t)k * a.state + n0 + n) * a.channels + c;
             a.hst[at] = h[n];
             if (BACK) a.gst[at] = R[n];
         }
+    if (n0) return;
     a.dsum[(int64_t)k * a.channels + c] = sum;
     if (c == 0) a.reset[k] = reset;
 }
 
 // Pass 2, in place: hst[k] (and, from the right, gst[k]) becomes the state that enters chunk k.  64 columns
 // by 16 segments of the chunks: each segment's own composition, then the ones before it, then the segment.
-// Eight chunks are loaded at a time: one after the other they are a chain of memory latencies.
+// Sixteen chunks are loaded at a time: one after the other they are a chain of memory latencies.
 template <typename T>
 __global__ __launch_bounds__(1024) void k_scan_carry(const Scan a) {
     __shared__ float sD[16][64], sH[16][64];
@@ -255,7 +279,7 @@ __global__ __launch_bounds__(1024) void k_scan_carry(const Scan a) {
     const float A2 = a.A[(int64_t)c * a.state + n] * SCAN_LOG2E;
     const int len = (a.n_chunks + 15) / 16;
     const int k0 = min(seg * len, a.n_chunks), k1 = min(k0 + len, a.n_chunks);
-    constexpr int BATCH = 8;
+    constexpr int BATCH = 16;
     float v[BATCH], dec[BATCH];
     int cut[BATCH];
     auto fetch = [&](int i0) {
@@ -316,13 +340,14 @@ __global__ __launch_bounds__(256) void k_scan_fwd(const Scan a) {
     const float skip = a.D ? a.D[c] : 0.0f;
 
     float A2[NP], h[NP];
-    load_rates<NP>(A2, a, c);
+    load_rates<NP>(A2, a, c, 0);
 #pragma unroll
     for (int n = 0; n < NP; ++n)
         h[n] = a.n_chunks > 1 && n < a.state ? a.hst[((int64_t)k * a.state + n) * a.channels + c] : 0.0f;
 
     Ahead<M, false> next;
-    next.load(a, r0, 0, len, c);
+    unsigned lane_bytes = (unsigned)c * sizeof(M);       // below 2^26 (2^24 channels)
+    next.load(a, r0, 0, len, lane_bytes);
     Stretch q = find_stretch(a.off, a.n_seqs, a.rows, r0, 0, len);
     for (int t0 = 0; t0 < len; t0 += SCAN_TILE) {
         const int t1 = min(t0 + SCAN_TILE, len);
@@ -335,25 +360,25 @@ __global__ __launch_bounds__(256) void k_scan_fwd(const Scan a) {
             const int t2 = uniform(min(t1, q.until));
             if (!q.inside) {
                 if (a.zero_rest && live)
-                    for (int i = t; i < t2; ++i) (y + (r0 + i) * a.y_stride)[(unsigned)c] = narrow<M>(0.0f);
+                    for (int i = t; i < t2; ++i) lane_at(y + (r0 + i) * a.y_stride, lane_bytes) = narrow<M>(0.0f);
                 t = t2;
-                if (t < len) next.load(a, r0, t, len, c);
+                if (t < len) next.load(a, r0, t, len, lane_bytes);
                 continue;
             }
             if (q.first) {
-                load_state<NP>(h, a.initial, a, q.s, c);
+                load_state<NP>(h, a.initial, a, q.s, c, 0);
                 q.first = false;
             }
             while (t < t2) {
                 const int from = t, count = uniform(min(AHEAD, t2 - t));
                 const Ahead<M, false> now = next;
                 t = uniform(t + count);
-                if (t < len) next.load(a, r0, t, len, c);
+                if (t < len) next.load(a, r0, t, len, lane_bytes);
                 float d[AHEAD], du[AHEAD], out[AHEAD];
+                steps_of<AHEAD>(d, a.softplus, now.delta, bias);
 #pragma unroll
                 for (int j = 0; j < AHEAD; ++j) {
                     const float uv = widen(now.u[j]);
-                    d[j] = step_of(a.softplus, now.delta[j], bias);
                     du[j] = d[j] * uv;
                     out[j] = skip * uv;
                 }
@@ -382,9 +407,10 @@ __global__ __launch_bounds__(256) void k_scan_fwd(const Scan a) {
                     after(at, h[NP / 2]);
                 }
                 if (live) {
+                    asm volatile("" : "+v"(lane_bytes));
 #pragma unroll
                     for (int j = 0; j < AHEAD; ++j)
-                        if (j < count) (y + (r0 + from + j) * a.y_stride)[(unsigned)c] = narrow<M>(out[j]);
+                        if (j < count) lane_at(y + (r0 + from + j) * a.y_stride, lane_bytes) = narrow<M>(out[j]);
                 }
             }
             if (a.final && q.last && t == q.until && live) store_state<NP>(a.final, h, a, q.s, c);
@@ -847,15 +873,20 @@ inline int padded_state(int state) {
     return np;
 }
 
+constexpr int SUM_STATES = 16;
+inline int sum_slices(int state) { return (int)ceil_div(state, SUM_STATES); }      // 1 up to sixteen states, whatever NP
+
 // Rows per chunk of the forward pass.  A chunk costs 16 bytes per state of traffic between the passes, so
-// long ones are preferred while they leave about four wavefronts for every SIMD (256 CUs x 4); up to 64
-// rows one pass without chunks is faster than three launches.
+// long ones are preferred while they leave about four wavefronts for every SIMD (256 CUs x 4).  Smaller problems
+// are bound by the time of one wavefront, which goes with its rows (0.6 us each), and take shorter chunks; up to
+// 32 rows one pass is faster than three launches.
 inline int scan_fwd_chunk(const mfcc_scan_args* a) {
-    if (a->rows <= 64) return 64;
+    if (a->rows <= 32) return 32;
     const int64_t waves = (int64_t)a->groups * ceil_div(a->channels / a->groups, WAVE);
     for (int chunk : {256, 128, 64})
         if (waves * ceil_div(a->rows, chunk) >= 4 * 1024) return chunk;
-    return 32;
+    if (waves * ceil_div(a->rows, 32) >= 768) return 32;
+    return waves * ceil_div(a->rows, 16) >= 1024 ? 16 : 8;
 }
 
 inline int bwd_channels_of(int np) { return 4 * WAVE / (np / 4); }
@@ -863,7 +894,7 @@ inline int scan_bwd_chunk(const mfcc_scan_args* a) {
     const int cpb = bwd_channels_of(padded_state(a->state)), most = cpb >= 256 ? 16 : cpb >= 128 ? 32 : 64;
     const int64_t blocks = (int64_t)a->groups * ceil_div(a->channels / a->groups, cpb);
     int chunk = most;
-    while (chunk > 16 && blocks * ceil_div(a->rows, chunk) < 1024) chunk /= 2;
+    while (chunk > 8 && blocks * ceil_div(a->rows, chunk) < 1024) chunk /= 2;
     return chunk;
 }
 
@@ -937,7 +968,9 @@ int scan_forward(const mfcc_scan_args* a, hipStream_t st) {
         const int rc = by_state(a->state, [&](auto np) {
             constexpr int NP = decltype(np)::value;
             if (f.n_chunks > 1) {
-                hipLaunchKernelGGL((k_scan_sum<T, NP, false>), dim3((unsigned)grid), dim3(block), 0, st, f);
+                if (grid * sum_slices(f.state) > 0x7fffff) return mfcc_detail::fail(MFCC_E_UNSUPPORTED, "batch too large: split it");
+                hipLaunchKernelGGL((k_scan_sum<T, std::min(NP, SUM_STATES), false>), dim3((unsigned)(grid * sum_slices(f.state))),
+                                   dim3(block), 0, st, f);
                 hipLaunchKernelGGL(k_scan_carry<T>, dim3((unsigned)ceil_div((int64_t)f.state * f.channels, 64), 1), dim3(1024),
                                    0, st, f);
             }
@@ -961,8 +994,9 @@ int scan_backward(const mfcc_scan_args* a, hipStream_t st) {
             f.blocks_per_group = (int)ceil_div(f.per, block);
             const int64_t grid = (int64_t)f.groups * f.blocks_per_group * f.n_chunks;
             if (f.n_chunks > 1) {
-                if (grid > 0x7fffff) return mfcc_detail::fail(MFCC_E_UNSUPPORTED, "batch too large: split it");
-                hipLaunchKernelGGL((k_scan_sum<T, NP, true>), dim3((unsigned)grid), dim3(block), 0, st, f);
+                if (grid * sum_slices(f.state) > 0x7fffff) return mfcc_detail::fail(MFCC_E_UNSUPPORTED, "batch too large: split it");
+                hipLaunchKernelGGL((k_scan_sum<T, std::min(NP, SUM_STATES), true>), dim3((unsigned)(grid * sum_slices(f.state))),
+                                   dim3(block), 0, st, f);
                 hipLaunchKernelGGL(k_scan_carry<T>, dim3((unsigned)ceil_div((int64_t)f.state * f.channels, 64), 2), dim3(1024),
                                    0, st, f);
             }

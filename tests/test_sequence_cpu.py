@@ -91,7 +91,7 @@ def test_workspaces_are_checked():
         assert fn(a, None) == _lib.MFCC_E_WORKSPACE
         a.d_workspace, a.workspace_bytes = None, need
         assert fn(a, None) == _lib.MFCC_E_WORKSPACE
-    assert lib.mfcc_selective_scan_workspace(scan_args(rows=64, **bufs)) == 0       # one pass, no chunks
+    assert lib.mfcc_selective_scan_workspace(scan_args(rows=32, **bufs)) == 0       # one pass, no chunks
     a = conv_args(rows=1000, d_x=16, d_dy=16, d_dx=16, d_dweight=16)
     need = lib.mfcc_causal_conv_backward_workspace(a)
     a.d_workspace, a.workspace_bytes = 256, need - 1
