@@ -873,8 +873,8 @@ inline int padded_state(int state) {
     return np;
 }
 
-constexpr int SUM_STATES = 16;
-inline int sum_slices(int state) { return (int)ceil_div(state, SUM_STATES); }      // 1 up to sixteen states, whatever NP
+constexpr int sum_states(bool back) { return back ? 8 : 16; }
+inline int sum_slices(int state, bool back) { return (int)ceil_div(state, sum_states(back)); }
 
 // Rows per chunk of the forward pass.  A chunk costs 16 bytes per state of traffic between the passes, so
 // long ones are preferred while they leave about four wavefronts for every SIMD (256 CUs x 4).  Smaller problems
@@ -968,8 +968,8 @@ int scan_forward(const mfcc_scan_args* a, hipStream_t st) {
         const int rc = by_state(a->state, [&](auto np) {
             constexpr int NP = decltype(np)::value;
             if (f.n_chunks > 1) {
-                if (grid * sum_slices(f.state) > 0x7fffff) return mfcc_detail::fail(MFCC_E_UNSUPPORTED, "batch too large: split it");
-                hipLaunchKernelGGL((k_scan_sum<T, std::min(NP, SUM_STATES), false>), dim3((unsigned)(grid * sum_slices(f.state))),
+                if (grid * sum_slices(f.state, false) > 0x7fffff) return mfcc_detail::fail(MFCC_E_UNSUPPORTED, "batch too large: split it");
+                hipLaunchKernelGGL((k_scan_sum<T, std::min(NP, sum_states(false)), false>), dim3((unsigned)(grid * sum_slices(f.state, false))),
                                    dim3(block), 0, st, f);
                 hipLaunchKernelGGL(k_scan_carry<T>, dim3((unsigned)ceil_div((int64_t)f.state * f.channels, 64), 1), dim3(1024),
                                    0, st, f);
@@ -994,8 +994,8 @@ int scan_backward(const mfcc_scan_args* a, hipStream_t st) {
             f.blocks_per_group = (int)ceil_div(f.per, block);
             const int64_t grid = (int64_t)f.groups * f.blocks_per_group * f.n_chunks;
             if (f.n_chunks > 1) {
-                if (grid * sum_slices(f.state) > 0x7fffff) return mfcc_detail::fail(MFCC_E_UNSUPPORTED, "batch too large: split it");
-                hipLaunchKernelGGL((k_scan_sum<T, std::min(NP, SUM_STATES), true>), dim3((unsigned)(grid * sum_slices(f.state))),
+                if (grid * sum_slices(f.state, true) > 0x7fffff) return mfcc_detail::fail(MFCC_E_UNSUPPORTED, "batch too large: split it");
+                hipLaunchKernelGGL((k_scan_sum<T, std::min(NP, sum_states(true)), true>), dim3((unsigned)(grid * sum_slices(f.state, true))),
                                    dim3(block), 0, st, f);
                 hipLaunchKernelGGL(k_scan_carry<T>, dim3((unsigned)ceil_div((int64_t)f.state * f.channels, 64), 2), dim3(1024),
                                    0, st, f);
