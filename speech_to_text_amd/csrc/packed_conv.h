@@ -452,8 +452,8 @@ __global__ __launch_bounds__(256) void k_conv_step(const ConvStep a) {
     for (int j = 0; j < K - 1; ++j) store_vec<M, VEC>(next + (int64_t)j * a.channels, win[j], n);
 }
 
-// Channels of a thread: four in every type.  With the eight that make 16 bytes in the 16-bit types the taps, sums
-// and rows in flight cost half the wavefronts (125 against 98 us for 30011 x 4096).
+// Channels of a thread.  With eight (16 bytes of a 16-bit type) the taps, sums and rows in flight cost half the
+// wavefronts (125 against 98 us for 30011 x 4096 in bfloat16).
 constexpr int CONV_VEC = 4;
 constexpr int CONV_AHEAD = 8;      // rows in flight of the forward pass
 

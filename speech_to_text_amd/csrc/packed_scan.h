@@ -803,59 +803,90 @@ struct ScanStep {
 };
 
 // Entries that name the same slot are successive tokens of that sequence and are taken by the first of
-// them; a slot outside the pool gives a zero row and touches no state.
-template <typename T, int NP>
+// them; a slot outside the pool gives a zero row and touches no state.  A thread has four states of a channel for
+// NE entries: their loads, which need the slots alone, go out together and before the list of slots is looked
+// through (a wavefront with one entry waits more than it moves: 3.2 TB/s), and A is read once for them.
+template <typename T, int NP, int NE>
 __global__ __launch_bounds__(256) void k_scan_step(const ScanStep a) {
     using M = typename T::mem;
     constexpr int LPC = NP / 4;
-    const int e0 = blockIdx.y;
-    int slot = e0;
-    bool again = false;
-    if (a.slots) {
-        slot = a.slots[e0];
-        const SlotUse use = slot_use(a.slots, a.batch, e0);
-        if (use.before && (unsigned)slot < (unsigned)a.n_slots) return;
-        again = use.after;
-    }
+    const int e0 = blockIdx.y * NE;
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int nq = (int)(id % LPC), n0 = nq * 4;
     const bool live = id / LPC < a.channels;
     const int c = live ? (int)(id / LPC) : 0;
-    M* y = static_cast<M*>(a.y) + c;
-    if ((unsigned)slot >= (unsigned)a.n_slots) {
-        if (live && nq == 0) y[(int64_t)e0 * a.y_stride] = narrow<M>(0.0f);
-        return;
-    }
     const int left = live ? max(a.state - n0, 0) : 0;           // of the lane's four states, how many exist
-    const int64_t at = ((int64_t)slot * a.channels + c) * a.state + n0;
+    int slot[NE];
+    bool in_pool[NE], again[NE] = {}, skipped[NE] = {};
+    int64_t at[NE];
+    float h[NE][4], A2[4], uv[NE], d[NE], b[NE][4], cv[NE][4];
+    M raw[NE];
     const int64_t bc = (int64_t)(c / a.per) * a.state + n0;
-    float h[4], A2[4];
-    load_vec<float, 4>(h, a.state_in + at, left);
-    load_vec<float, 4>(A2, a.A + (int64_t)c * a.state + n0, left);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) A2[i] *= SCAN_LOG2E;
+    for (int k = 0; k < NE; ++k) {
+        const int e = min(e0 + k, a.batch - 1);
+        slot[k] = a.slots ? a.slots[e] : e;
+        in_pool[k] = (unsigned)slot[k] < (unsigned)a.n_slots && e0 + k < a.batch;
+    }
+#pragma unroll
+    for (int k = 0; k < NE; ++k) {
+        at[k] = ((int64_t)(in_pool[k] ? slot[k] : 0) * a.channels + c) * a.state + n0;
+        load_vec<float, 4>(h[k], a.state_in + at[k], in_pool[k] ? left : 0);
+    }
+    auto token = [&](int k, int e) {                            // the inputs of entry e
+        uv[k] = widen(static_cast<const M*>(a.u)[(int64_t)e * a.u_stride + c]);
+        raw[k] = static_cast<const M*>(a.delta)[(int64_t)e * a.delta_stride + c];
+        load_vec<M, 4>(b[k], static_cast<const M*>(a.B) + (int64_t)e * a.B_stride + bc, left);
+        load_vec<M, 4>(cv[k], static_cast<const M*>(a.C) + (int64_t)e * a.C_stride + bc, left);
+    };
+#pragma unroll
+    for (int k = 0; k < NE; ++k) token(k, min(e0 + k, a.batch - 1));
+    load_vec<float, 4>(A2, a.A + (int64_t)c * a.state + n0, left);
     const float bias = a.bias ? a.bias[c] : 0.0f, skip = a.D ? a.D[c] : 0.0f;
-    for (int e = e0; e < a.batch; ++e) {
-        if (e != e0) {
-            if (!again) break;
-            if (a.slots[e] != slot) continue;
+    if (a.slots) {
+        for (int i = threadIdx.x & 63; i < a.batch; i += WAVE) {
+            const int other = a.slots[i];
+#pragma unroll
+            for (int k = 0; k < NE; ++k) {
+                skipped[k] |= other == slot[k] && i < e0 + k;
+                again[k] |= other == slot[k] && i > e0 + k;
+            }
         }
-        const float uv = widen(static_cast<const M*>(a.u)[(int64_t)e * a.u_stride + c]);
-        const float d = step_of(a.softplus, static_cast<const M*>(a.delta)[(int64_t)e * a.delta_stride + c], bias);
-        float b[4], cc[4];
-        load_vec<M, 4>(b, static_cast<const M*>(a.B) + (int64_t)e * a.B_stride + bc, left);
-        load_vec<M, 4>(cc, static_cast<const M*>(a.C) + (int64_t)e * a.C_stride + bc, left);
+#pragma unroll
+        for (int k = 0; k < NE; ++k) { skipped[k] = __ballot(skipped[k]) != 0; again[k] = __ballot(again[k]) != 0; }
+    }
+#pragma unroll
+    for (int n = 0; n < 4; ++n) A2[n] *= SCAN_LOG2E;
+    M* y = static_cast<M*>(a.y) + c;
+    auto advance = [&](int k, int e) {
+        d[k] = step_of(a.softplus, raw[k], bias);
         float acc = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            h[i] = fmaf(exp2_hw(d * A2[i]), h[i], d * uv * b[i]);
-            acc = fmaf(cc[i], h[i], acc);
+        for (int n = 0; n < 4; ++n) {
+            h[k][n] = fmaf(exp2_hw(d[k] * A2[n]), h[k][n], d[k] * uv[k] * b[k][n]);
+            acc = fmaf(cv[k][n], h[k][n], acc);
         }
         acc = sum_states<LPC>(acc);
-        if (a.D) acc = fmaf(skip, uv, acc);
+        if (a.D) acc = fmaf(skip, uv[k], acc);
         if (live && nq == 0) y[(int64_t)e * a.y_stride] = narrow<M>(acc);
+    };
+#pragma unroll
+    for (int k = 0; k < NE; ++k) {
+        if (e0 + k >= a.batch) break;
+        if (!in_pool[k]) {
+            if (live && nq == 0) y[(int64_t)(e0 + k) * a.y_stride] = narrow<M>(0.0f);
+            continue;
+        }
+        if (skipped[k]) continue;
+        advance(k, e0 + k);
+        if (again[k])
+            for (int e = e0 + k + 1; e < a.batch; ++e)
+                if (a.slots[e] == slot[k]) {
+                    token(k, e);
+                    advance(k, e);
+                }
+        if (left > 0) store_vec<float, 4>(a.state_out + at[k], h[k], left);
     }
-    if (left > 0) store_vec<float, 4>(a.state_out + at, h, left);
 }
 
 // ---- host ------------------------------------------------------------------------------------------------
@@ -1036,8 +1067,12 @@ int scan_step(const mfcc_scan_args* a, int n_slots, const int32_t* slots, hipStr
     f.channels = a->channels; f.state = a->state; f.per = a->channels / a->groups; f.softplus = a->softplus;
     return by_state(a->state, [&](auto np) {
         constexpr int NP = decltype(np)::value;
-        hipLaunchKernelGGL((k_scan_step<T, NP>), dim3((unsigned)ceil_div((int64_t)a->channels * (NP / 4), 256), (unsigned)f.batch),
-                           dim3(256), 0, st, f);
+        const int64_t tiles = ceil_div((int64_t)a->channels * (NP / 4), 256);
+        // four entries per thread once that still leaves sixteen wavefronts for every SIMD
+        if (tiles * f.batch >= 4 * 16 * 256)
+            hipLaunchKernelGGL((k_scan_step<T, NP, 4>), dim3((unsigned)tiles, (unsigned)ceil_div(f.batch, 4)), dim3(256), 0, st, f);
+        else
+            hipLaunchKernelGGL((k_scan_step<T, NP, 1>), dim3((unsigned)tiles, (unsigned)f.batch), dim3(256), 0, st, f);
         PACKED_LAUNCHED();
         return (int)MFCC_OK;
     });
