@@ -218,14 +218,16 @@ __device__ __forceinline__ float halve16(float x, float y) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// Sum over the 64 lanes, in every lane.
-__device__ __forceinline__ float wave_sum(float v) {
+// Sum over 16, 32 or (any larger COUNT) 64 neighbouring lanes, in every one of them.
+template <int COUNT>
+__device__ __forceinline__ float lanes_sum(float v) {
     v += dpp<0xB1>(v);          // quad_perm [1, 0, 3, 2]
     v += dpp<0x4E>(v);          // quad_perm [2, 3, 0, 1]
     v += dpp<0x141>(v);         // row_half_mirror
     v += dpp<0x140>(v);         // row_mirror
-    v = halve16(v, v);
-    return halve32(v, v);
+    if (COUNT >= 32) v = halve16(v, v);
+    if (COUNT >= 64) v = halve32(v, v);
+    return v;
 }
 
 // Whether another entry of a batch names the slot of entry e0, before or after it.  Every wavefront looks

@@ -3,7 +3,7 @@
 //   gate:  y = norm(x silu(z)) w + b  or  (norm(x) w + b) silu(z), over `groups` slices of the row
 //   norm:  v / sqrt(mean(v^2) + eps), of v - mean(v) for the layer form.
 // Bound by memory: every row is read once, held in registers (eight neighbouring elements a thread and
-// step), reduced over 64, 256 or 1024 threads and written once.  The layer form's deviation is summed
+// step), reduced over 16 to 1024 threads and written once.  The layer form's deviation is summed
 // around the mean, from the registers.
 #pragma once
 #include "packed.h"
@@ -11,6 +11,9 @@
 namespace packed {
 
 constexpr int NV = 8;
+
+// Threads of a workgroup: several rows within wavefronts, or one row of several wavefronts.
+constexpr int norm_block(int threads_per_row) { return threads_per_row <= WAVE ? 256 : threads_per_row; }
 
 struct Norm {
     const void *x, *z, *residual, *r_in, *dy, *dr;
@@ -26,7 +29,7 @@ struct Norm {
 // Sums of two values over the TPU threads of a unit.
 template <int TPU>
 __device__ __forceinline__ void unit_sum2(float& a, float& b, float (*sh)[2]) {
-    a = wave_sum(a); b = wave_sum(b);
+    a = lanes_sum<TPU>(a); b = lanes_sum<TPU>(b);
     if (TPU > WAVE) {
         constexpr int W = TPU / WAVE;
         const int wave = threadIdx.x >> 6;
@@ -49,13 +52,13 @@ __device__ __forceinline__ void load_or(float (&v)[NV], const M* p, int n, float
 }
 
 template <typename T, typename RT, bool GATE, int TPU, int IT>
-__global__ __launch_bounds__(TPU < 256 ? 256 : TPU) void k_norm_fwd(const Norm a) {
+__global__ __launch_bounds__(norm_block(TPU)) void k_norm_fwd(const Norm a) {
     using M = typename T::mem;
     using RM = typename RT::mem;
-    constexpr int PER = TPU < 256 ? 256 / TPU : 1;
+    constexpr int PER = norm_block(TPU) / TPU;
     __shared__ float sh[TPU > WAVE ? TPU / WAVE : 1][2];
     const int64_t unit = (int64_t)blockIdx.x * PER + (PER > 1 ? threadIdx.x / TPU : 0);
-    if (unit >= a.rows * a.groups) return;                    // whole wavefronts of a one-wavefront unit
+    if (unit >= a.rows * a.groups) return;                    // the sums of a smaller unit stay in its own lanes
     const int64_t row = a.groups > 1 ? unit / a.groups : unit;
     const int c_base = a.groups > 1 ? (int)(unit % a.groups) * a.width : 0;
     const int tid = PER > 1 ? threadIdx.x % TPU : threadIdx.x;
@@ -122,40 +125,83 @@ __global__ __launch_bounds__(TPU < 256 ? 256 : TPU) void k_norm_fwd(const Norm a
 }
 
 // A block keeps its columns and walks over rows; the sums over rows stay in registers until its end, then
-// one partial row per block is written and k_norm_reduce adds those in a fixed order.
+// one partial row per block is written and k_norm_reduce adds those in a fixed order.  With eight elements a thread
+// (IT = 1) the tables stay in registers and the next row is in flight during the reductions of the current one (for
+// the gate in 16-bit types only: three float32 rows ahead cost a wavefront per SIMD, 28 against 26 us at 4099 x 1537).
 template <typename T, typename RT, bool GATE, int TPU, int IT>
-__global__ __launch_bounds__(TPU < 256 ? 256 : TPU) void k_norm_bwd(const Norm a) {
+__global__ __launch_bounds__(norm_block(TPU)) void k_norm_bwd(const Norm a) {
     using M = typename T::mem;
     using RM = typename RT::mem;
-    constexpr int PER = TPU < 256 ? 256 / TPU : 1;
+    constexpr int PER = norm_block(TPU) / TPU;
+    constexpr bool HELD = IT == 1, AHEAD_ROW = HELD && (!GATE || sizeof(M) == 2);
     __shared__ float sh[TPU > WAVE ? TPU / WAVE : 1][2];
     __shared__ float fold[PER > 1 ? PER : 1][PER > 1 ? TPU * NV : 1];
     const int slot = PER > 1 ? threadIdx.x / TPU : 0, tid = PER > 1 ? threadIdx.x % TPU : threadIdx.x;
     const int c_base = blockIdx.y * a.width;
     float dw[IT][NV] = {}, db[IT][NV] = {}, ds[GATE ? 1 : IT][NV] = {};
+    auto left = [&](int k) { return max(a.width - (k * TPU + tid) * NV, 0); };
+    auto col = [&](int k) { return c_base + (k * TPU + tid) * NV; };
 
-    for (int64_t row = (int64_t)blockIdx.x * PER + slot; row < a.rows; row += (int64_t)gridDim.x * PER) {
-        float v[IT][NV], dn[IT][NV], s1 = 0.0f, s2 = 0.0f, t1 = 0.0f, t2 = 0.0f;
-        float xv[IT][NV], zv[GATE ? IT : 1][NV], dyv[IT][NV];
+    // what a row is made of: dy, and x and z (gate) or r, dr and x (add)
+    struct RowIn { Raw<M, NV> dy[IT], x[IT], z[GATE ? IT : 1]; Raw<RM, NV> r[GATE ? 1 : IT], dr[GATE ? 1 : IT]; };
+    auto fetch = [&](RowIn& in, int64_t row) {
+        const float zero[NV] = {};
 #pragma unroll
         for (int k = 0; k < IT; ++k) {
-            const int w0 = (k * TPU + tid) * NV, c = c_base + w0, n = max(a.width - w0, 0);
-            load_or<M>(dyv[k], a.dy ? static_cast<const M*>(a.dy) + row * a.dy_stride + c : nullptr, n, 0.0f);
-            float w[NV];
-            load_or<float>(w, a.weight ? a.weight + c : nullptr, n, 1.0f);
+            const int c = col(k), n = left(k);
+            if (a.dy) load_raw<M, NV>(in.dy[k], static_cast<const M*>(a.dy) + row * a.dy_stride + c, n);
+            else in.dy[k].set(zero);
+            if (GATE || a.x) load_raw<M, NV>(in.x[k], static_cast<const M*>(a.x) + row * a.x_stride + c, n);
             if (GATE) {
-                load_vec<M, NV>(xv[k], static_cast<const M*>(a.x) + row * a.x_stride + c, n);
-                load_vec<M, NV>(zv[k], static_cast<const M*>(a.z) + row * a.z_stride + c, n);
-#pragma unroll
-                for (int i = 0; i < NV; ++i) {
-                    const float gate = zv[k][i] * sigmoid_f(zv[k][i]);
-                    v[k][i] = a.gate_first ? xv[k][i] * gate : xv[k][i];
-                    dn[k][i] = (a.gate_first ? dyv[k][i] : dyv[k][i] * gate) * w[i];
-                }
+                load_raw<M, NV>(in.z[GATE ? k : 0], static_cast<const M*>(a.z) + row * a.z_stride + c, n);
             } else {
-                load_vec<RM, NV>(v[k], static_cast<const RM*>(a.r_in) + row * a.r_stride + c, n);
+                load_raw<RM, NV>(in.r[GATE ? 0 : k], static_cast<const RM*>(a.r_in) + row * a.r_stride + c, n);
+                if (a.dr) load_raw<RM, NV>(in.dr[GATE ? 0 : k], static_cast<const RM*>(a.dr) + row * a.dr_stride + c, n);
+                else in.dr[GATE ? 0 : k].set(zero);
+            }
+        }
+    };
+    // weight, and the bias (gate) or the scale (add)
+    float w[IT][NV], t[IT][NV];
+    auto tables = [&]() {
 #pragma unroll
-                for (int i = 0; i < NV; ++i) dn[k][i] = dyv[k][i] * w[i];
+        for (int k = 0; k < IT; ++k) {
+            const int c = col(k), n = left(k);
+            load_or<float>(w[k], a.weight ? a.weight + c : nullptr, n, 1.0f);
+            if (GATE) load_or<float>(t[k], a.bias ? a.bias + c : nullptr, n, 0.0f);
+            else load_or<float>(t[k], a.scale ? a.scale + c : nullptr, n, a.scale_value);
+        }
+    };
+    if (HELD) tables();
+
+    const int64_t step = (int64_t)gridDim.x * PER;
+    int64_t row = (int64_t)blockIdx.x * PER + slot;
+    RowIn next;
+    if (AHEAD_ROW && row < a.rows) fetch(next, row);
+    for (; row < a.rows; row += step) {
+        RowIn in;
+        if (AHEAD_ROW) {
+            in = next;
+            if (row + step < a.rows) fetch(next, row + step);
+        } else {
+            fetch(in, row);
+            if (!HELD) tables();
+        }
+        float v[IT][NV], dn[IT][NV], s1 = 0.0f, s2 = 0.0f, t1 = 0.0f, t2 = 0.0f;
+#pragma unroll
+        for (int k = 0; k < IT; ++k) {
+            const int n = left(k);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const float dy = in.dy[k].get(i);
+                if (GATE) {
+                    const float z = in.z[GATE ? k : 0].get(i), x = in.x[k].get(i), gate = z * sigmoid_f<sizeof(M) == 4>(z);
+                    v[k][i] = a.gate_first ? x * gate : x;
+                    dn[k][i] = (a.gate_first ? dy : dy * gate) * w[k][i];
+                } else {
+                    v[k][i] = in.r[GATE ? 0 : k].get(i);
+                    dn[k][i] = dy * w[k][i];
+                }
             }
             if (n < NV) {
 #pragma unroll
@@ -174,7 +220,7 @@ __global__ __launch_bounds__(TPU < 256 ? 256 : TPU) void k_norm_bwd(const Norm a
             s2 = t2 = 0.0f;
 #pragma unroll
             for (int k = 0; k < IT; ++k) {
-                const int n = a.width - (k * TPU + tid) * NV;
+                const int n = left(k);
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
                     const float d = i < n ? v[k][i] - mean : 0.0f;
@@ -188,7 +234,7 @@ __global__ __launch_bounds__(TPU < 256 ? 256 : TPU) void k_norm_bwd(const Norm a
         const float proj = t2 * a.inv_width * q;                 // mean(dn * v q)
 #pragma unroll
         for (int k = 0; k < IT; ++k) {
-            const int w0 = (k * TPU + tid) * NV, c = c_base + w0, n = a.width - w0;
+            const int c = col(k), n = left(k);
             if (n <= 0) continue;
             float dv[NV];
 #pragma unroll
@@ -199,14 +245,13 @@ __global__ __launch_bounds__(TPU < 256 ? 256 : TPU) void k_norm_bwd(const Norm a
             }
             const int64_t at = row * a.channels + c;
             if (GATE) {
-                float dz[NV], w[NV], b[NV];
-                load_or<float>(w, a.weight ? a.weight + c : nullptr, n, 1.0f);
-                load_or<float>(b, a.bias ? a.bias + c : nullptr, n, 0.0f);
+                float dz[NV];
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
-                    const float z = zv[k][i], sg = sigmoid_f(z), gate = z * sg, slope = sg * fmaf(z, 1.0f - sg, 1.0f);
-                    const float body = a.gate_first ? dyv[k][i] : dyv[k][i] * gate;
-                    dz[i] = (a.gate_first ? dv[i] * xv[k][i] : dyv[k][i] * fmaf(v[k][i], w[i], b[i])) * slope;
+                    const float z = in.z[GATE ? k : 0].get(i), x = in.x[k].get(i), dy = in.dy[k].get(i);
+                    const float sg = sigmoid_f<sizeof(M) == 4>(z), gate = z * sg, slope = sg * fmaf(z, 1.0f - sg, 1.0f);
+                    const float body = a.gate_first ? dy : dy * gate;
+                    dz[i] = (a.gate_first ? dv[i] * x : dy * fmaf(v[k][i], w[k][i], t[k][i])) * slope;
                     if (a.gate_first) dv[i] *= gate;
                     dw[k][i] = fmaf(body, v[k][i], dw[k][i]);
                     db[k][i] += body;
@@ -214,22 +259,21 @@ __global__ __launch_bounds__(TPU < 256 ? 256 : TPU) void k_norm_bwd(const Norm a
                 store_vec<M, NV>(static_cast<M*>(a.dx) + at, dv, n);
                 store_vec<M, NV>(static_cast<M*>(a.dz) + at, dz, n);
             } else {
-                float dr[NV];
-                load_or<RM>(dr, a.dr ? static_cast<const RM*>(a.dr) + row * a.dr_stride + c : nullptr, n, 0.0f);
-                if (a.x) load_vec<M, NV>(xv[k], static_cast<const M*>(a.x) + row * a.x_stride + c, n);
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
-                    dv[i] += dr[i];
-                    dw[k][i] = fmaf(dyv[k][i], v[k][i], dw[k][i]);
-                    db[k][i] += dyv[k][i];
-                    if (a.x) ds[k][i] = fmaf(dv[i], xv[k][i], ds[k][i]);
+                    const float dy = in.dy[k].get(i);
+                    dv[i] += in.dr[GATE ? 0 : k].get(i);
+                    dw[k][i] = fmaf(dy, v[k][i], dw[k][i]);
+                    db[k][i] += dy;
+                }
+                if (a.x) {
+#pragma unroll
+                    for (int i = 0; i < NV; ++i) ds[GATE ? 0 : k][i] = fmaf(dv[i], in.x[k].get(i), ds[GATE ? 0 : k][i]);
                 }
                 if (a.dresidual) store_vec<RM, NV>(static_cast<RM*>(a.dresidual) + at, dv, n);
                 if (a.dx) {
-                    float sc[NV];
-                    load_or<float>(sc, a.scale ? a.scale + c : nullptr, n, a.scale_value);
 #pragma unroll
-                    for (int i = 0; i < NV; ++i) dv[i] *= sc[i];
+                    for (int i = 0; i < NV; ++i) dv[i] *= t[k][i];
                     store_vec<M, NV>(static_cast<M*>(a.dx) + at, dv, n);
                 }
             }
@@ -249,10 +293,10 @@ __global__ __launch_bounds__(TPU < 256 ? 256 : TPU) void k_norm_bwd(const Norm a
                 for (int i = 0; i < NV; ++i) fold[slot][i * TPU + tid] = s[i];
                 __syncthreads();
                 for (int e = threadIdx.x; e < TPU * NV; e += 256) {
-                    float t = 0.0f;
+                    float f = 0.0f;
 #pragma unroll
-                    for (int p = 0; p < PER; ++p) t += fold[p][(e % NV) * TPU + e / NV];
-                    if (k * TPU * NV + e < a.width) out[k * TPU * NV + e] = t;
+                    for (int p = 0; p < PER; ++p) f += fold[p][(e % NV) * TPU + e / NV];
+                    if (e < a.width) out[e] = f;
                 }
             } else if (w0 < a.width) {
                 store_vec<float, NV>(out + w0, s, a.width - w0);
@@ -282,23 +326,26 @@ __global__ __launch_bounds__(1024) void k_norm_reduce(const float* __restrict__ 
 // ---- host --------------------------------------------------------------------------------------------
 constexpr int NORM_MAX_WIDTH = 32768;
 
-// Threads per row and steps of eight elements per thread: (64, 1) .. (1024, 4).
+// Threads per row and steps of eight elements per thread: (16, 1) .. (1024, 4).
 template <typename Fn>
 int by_width_of_row(int width, Fn&& fn) {
     using std::integral_constant;
+    if (width <= 128) return fn(integral_constant<int, 16>{}, integral_constant<int, 1>{});
+    if (width <= 256) return fn(integral_constant<int, 32>{}, integral_constant<int, 1>{});
     if (width <= 512) return fn(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+    if (width <= 1024) return fn(integral_constant<int, 128>{}, integral_constant<int, 1>{});
     if (width <= 2048) return fn(integral_constant<int, 256>{}, integral_constant<int, 1>{});
     if (width <= 4096) return fn(integral_constant<int, 256>{}, integral_constant<int, 2>{});
-    if (width <= 8192) return fn(integral_constant<int, 1024>{}, integral_constant<int, 1>{});
+    if (width <= 8192) return fn(integral_constant<int, 512>{}, integral_constant<int, 2>{});
     if (width <= 16384) return fn(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
     return fn(integral_constant<int, 1024>{}, integral_constant<int, 4>{});
 }
 
-// Blocks that walk over the rows in the backward pass: four of 256 threads for each of the 256 CUs.
+// Blocks that walk over the rows in the backward pass: about four wavefronts for each of the 1024 SIMDs.
 inline int norm_bwd_blocks(const mfcc_norm_args* a) {
-    const int width = a->channels / a->groups, per = width <= 512 ? 4 : 1;
-    const int64_t most = std::max<int64_t>(1, (width <= 4096 ? 1024 : 512) / a->groups);
-    return (int)std::min<int64_t>(ceil_div(a->rows, per), most);
+    const int width = a->channels / a->groups, per = width <= 128 ? 16 : width <= 256 ? 8 : width <= 512 ? 4 : 1;
+    const int64_t blocks = width <= 512 ? 1024 : width <= 1024 ? 2048 : width <= 4096 ? 1024 : 512;
+    return (int)std::min<int64_t>(ceil_div(a->rows, per), std::max<int64_t>(1, blocks / a->groups));
 }
 
 inline Norm norm_args(const mfcc_norm_args* a) {
@@ -318,10 +365,10 @@ int norm_forward(const mfcc_norm_args* a, hipStream_t st) {
     if (a->rows == 0) return MFCC_OK;
     const Norm f = norm_args(a);
     return by_width_of_row(f.width, [&](auto tpu, auto it) {
-        constexpr int TPU = decltype(tpu)::value, IT = decltype(it)::value, PER = TPU < 256 ? 256 / TPU : 1;
+        constexpr int TPU = decltype(tpu)::value, IT = decltype(it)::value, PER = norm_block(TPU) / TPU;
         const int64_t blocks = ceil_div(f.rows * f.groups, PER);
         if (blocks > 0x3fffff) return mfcc_detail::fail(MFCC_E_UNSUPPORTED, "batch too large: split it");
-        hipLaunchKernelGGL((k_norm_fwd<T, RT, GATE, TPU, IT>), dim3((unsigned)blocks), dim3(TPU < 256 ? 256 : TPU), 0, st, f);
+        hipLaunchKernelGGL((k_norm_fwd<T, RT, GATE, TPU, IT>), dim3((unsigned)blocks), dim3(norm_block(TPU)), 0, st, f);
         PACKED_LAUNCHED();
         return (int)MFCC_OK;
     });
@@ -338,7 +385,7 @@ int norm_backward(const mfcc_norm_args* a, hipStream_t st) {
         constexpr int TPU = decltype(tpu)::value, IT = decltype(it)::value;
         if (blocks > 0) {
             hipLaunchKernelGGL((k_norm_bwd<T, RT, GATE, TPU, IT>), dim3((unsigned)blocks, (unsigned)f.groups),
-                               dim3(TPU < 256 ? 256 : TPU), 0, st, f);
+                               dim3(norm_block(TPU)), 0, st, f);
             PACKED_LAUNCHED();
         }
         if (sums) {
