@@ -358,7 +358,10 @@ def test_scan_extreme_steps(gpu):
 
 
 # ---- norms ---------------------------------------------------------------------------------------------------------
-NORMS = [(1, 1), (3, 7), (9, 64), (5, 513), (2, 1000), (70, 96), (4, 2049), (3, 4100), (2, 9001), (1, 20000), (300, 40)]
+NORMS = [(1, 1), (3, 7), (9, 64), (5, 513), (2, 1000), (70, 96), (4, 2049), (3, 4100), (2, 9001), (1, 20000), (300, 40),
+         (6, 1500), (77, 200), (3, 7000),
+         # rows enough that a workgroup of the gradient kernels walks over several, for each number of threads per row
+         (20000, 24), (9000, 130), (4500, 300), (2500, 1100), (2300, 600)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -486,6 +489,125 @@ def test_norms_of_special_rows(gpu):
     assert S.gate_norm(none, none).shape == (0, 99) and S.add_norm(none, none)[0].shape == (0, 99)
     assert (S.gate_norm_backward(none, none, none, w).weight == 0).all()
     assert (S.add_norm_backward(none, None, none, w).weight == 0).all()
+
+
+# ---- every choice of tile and chunk ------------------------------------------------------------------------------------
+def scan64(u, d, A, B, C, dy, off, rate):
+    """Values and gradients row by row in 64 bits on the GPU; `rate` is A, or |A| for magnitudes (d u, B, C, dy then
+    positive as well)."""
+    rows, ch = u.shape
+    n = A.shape[1]
+    y, du, dd, dB, dC = (torch.zeros_like(t) for t in (u, u, d, B, C))
+    dA = torch.zeros_like(A)
+    for lo, hi in zip(off[:-1], off[1:]):
+        hs = torch.zeros(hi - lo + 1, ch, n, dtype=torch.float64, device=u.device)
+        for t in range(lo, hi):
+            hs[t - lo + 1] = torch.exp(d[t, :, None] * A) * hs[t - lo] + (d[t] * u[t])[:, None] * B[t]
+            y[t] = (hs[t - lo + 1] * C[t]).sum(1)
+        carry = torch.zeros(ch, n, dtype=torch.float64, device=u.device)
+        for t in range(hi - 1, lo - 1, -1):
+            dC[t] = (hs[t - lo + 1] * dy[t, :, None]).sum(0)
+            g = carry + dy[t, :, None] * C[t]
+            dB[t] = (g * (d[t] * u[t])[:, None]).sum(0)
+            carry = g * torch.exp(d[t, :, None] * A)
+            gB, w = (g * B[t]).sum(1), carry * hs[t - lo]
+            dA += w * d[t, :, None]
+            dd[t], du[t] = u[t] * gB + (w * rate).sum(1), d[t] * gB
+    return dict(y=y, u=du, delta=dd, A=dA, B=dB, C=dC)
+
+
+@pytest.mark.parametrize("rows,ch,n", [
+    (16500, 4096, 1), (8300, 4096, 2), (4200, 4096, 3), (1500, 704, 4), (900, 700, 5),     # forward 256, 128, 64, 16 and 8 rows
+    (1100, 4096, 16), (2100, 1024, 16), (1600, 1024, 16), (1200, 640, 16)])                # gradient 64, 32, 16 and 8; forward 32
+def test_scan_of_every_chunk_length(gpu, rows, ch, n):
+    import speech_to_text_amd as S
+
+    g = gen(gpu, rows)
+    cuts = [0, 37, rows // 3, rows // 3 + 1, rows - 300, rows]
+    u, dy = randn(g, rows, ch, dtype=BF16), randn(g, rows, ch, dtype=BF16)
+    delta = rand(g, rows, ch, lo=0.01, hi=0.1).to(BF16)
+    B, C = randn(g, rows, n, dtype=BF16), randn(g, rows, n, dtype=BF16)
+    A = -rand(g, ch, n, lo=0.5, hi=2.0)
+    off = torch.tensor(cuts, dtype=torch.int64, device=gpu)
+    y = S.selective_scan(u, delta, A, B, C, None, None, off)
+    gr = S.selective_scan_backward(dy, u, delta, A, B, C, None, None, off)
+    up = lambda *ts: [t.double() for t in ts]
+    ud, dd, Ad, Bd, Cd, dyd = up(u, delta, A, B, C, dy)
+    want = scan64(ud, dd, Ad, Bd, Cd, dyd, cuts, Ad)
+    size = scan64(ud.abs(), dd, Ad, Bd.abs(), Cd.abs(), dyd.abs(), cuts, Ad.abs())
+    # |d A| < 0.2 and A d > 0.005 on average 0.07: a state forgets within some hundred rows; (4 + 12 |d A|) roundings for
+    # each of those, and the chunk's own sum of d
+    steps = 7 * 400
+    for name, got in dict(y=y, u=gr.u, delta=gr.delta, A=gr.A, B=gr.B, C=gr.C).items():
+        kind = F32 if name == "A" else BF16
+        extra = dict(A=rows, B=ch, C=ch).get(name, 0)
+        R.assert_close(got, want[name].cpu(), kind, size[name].cpu(), steps + extra, name)
+
+
+@pytest.mark.parametrize("rows", [9000, 17000, 34000, 66000])
+def test_causal_conv_of_every_tile(gpu, rows):
+    """Sizes at which a thread of the forward pass takes 16, 32, 64 and 128 rows, of the gradient 32, 64 and 128."""
+    import speech_to_text_amd as S
+
+    g = gen(gpu, rows)
+    ch, k = 4096, 4
+    x = torch.empty(rows, ch, dtype=BF16, device=gpu).normal_(generator=g)
+    dy = torch.empty(rows, ch, dtype=BF16, device=gpu).normal_(generator=g)
+    w, b = randn(g, ch, k, scale=0.5), randn(g, ch, scale=0.3)
+    cuts = [0, 3, 131, rows // 2, rows // 2 + 2, rows - 1000, rows]
+    off = torch.tensor(cuts, dtype=torch.int64, device=gpu)
+    y = S.causal_conv(x, w, b, off, activation="silu")
+    gr = S.causal_conv_backward(dy, x, w, b, off, activation="silu")
+    dw, db = torch.zeros(ch, k, dtype=torch.float64, device=gpu), torch.zeros(ch, dtype=torch.float64, device=gpu)
+    biggest = 0.0
+    for lo, hi in zip(cuts[:-1], cuts[1:]):
+        line = torch.cat([torch.zeros(k - 1, ch, dtype=torch.float64, device=gpu), x[lo:hi].double()])
+        p = sum(line[j:j + hi - lo] * w[:, j].double() for j in range(k)) + b.double()
+        size = sum(line[j:j + hi - lo].abs() * w[:, j].double().abs() for j in range(k)) + b.double().abs()
+        sg = torch.sigmoid(p)
+        dp = dy[lo:hi].double() * sg * (1 + p * (1 - sg))
+        dw += torch.stack([(dp * line[j:j + hi - lo]).sum(0) for j in range(k)], 1)
+        db += dp.sum(0)
+        biggest = max(biggest, float((dp.abs() * (1 + size)).max()))
+        late = torch.cat([dp, torch.zeros(k - 1, ch, dtype=torch.float64, device=gpu)])
+        dx = sum(late[k - 1 - j:k - 1 - j + hi - lo] * w[:, j].double() for j in range(k))
+        reach = sum(late[k - 1 - j:k - 1 - j + hi - lo].abs() * w[:, j].double().abs() for j in range(k))
+        for name, got, want, mag in (("y", y, p * sg, size), ("x", gr.x, dx, reach + dy[lo:hi].double().abs().max() * size)):
+            # sigmoid without its second exponent word: |p| more roundings, |p| < 16
+            limit = 2.0 ** -8 * want.abs() + 2.0 ** -126 + 40 * 2.0 ** -24 * mag
+            assert ((got[lo:hi].double() - want).abs() <= limit).all(), (name, lo)
+    for got, want in ((gr.weight, dw), (gr.bias, db)):
+        assert (got.double() - want).abs().max() <= (rows + 40) * 2.0 ** -24 * biggest * 6
+
+
+def test_scan_step_of_many_entries(gpu):
+    """Enough entries that a thread takes four; some slots named again, near and far; padded rows at the end."""
+    import speech_to_text_amd as S
+
+    g = gen(gpu, 31)
+    m, ch, n, pool = 1103, 1024, 16, 1200
+    slots = torch.randperm(pool, generator=g, device=gpu)[:m].to(torch.int32)
+    slots[1] = slots[0]
+    slots[7], slots[9], slots[1000] = slots[4], slots[4], slots[4]
+    slots[1098:] = -1
+    u, delta = randn(g, m, ch), rand(g, m, ch, hi=0.3)
+    A, B, C, D = -rand(g, ch, n, lo=0.1, hi=1.0), randn(g, m, n), randn(g, m, n), randn(g, ch)
+    state = randn(g, pool, ch, n)
+    want, size = state.double(), state.double().abs()
+    got_state = state.clone()
+    y = S.selective_scan_step(u, delta, A, B, C, got_state, D, slots=slots)
+    for i, slot in enumerate(slots.tolist()):
+        if slot < 0:
+            assert (y[i] == 0).all()
+            continue
+        decay = torch.exp(delta[i].double()[:, None] * A.double())
+        step = (delta[i].double() * u[i].double())[:, None]
+        want[slot] = decay * want[slot] + step * B[i].double()
+        size[slot] = decay * size[slot] + step.abs() * B[i].double().abs()
+        wy = (want[slot] * C[i].double()).sum(1) + D.double() * u[i].double()
+        ws = (size[slot] * C[i].double().abs()).sum(1) + D.double().abs() * u[i].double().abs()
+        assert ((y[i].double() - wy).abs() <= (16 * 4 + n) * 2.0 ** -24 * ws).all(), i     # at most four tokens of a slot
+    assert ((got_state.double() - want).abs() <= 16 * 4 * 2.0 ** -24 * size).all()
 
 
 # ---- empty batches, offsets, streams, graphs --------------------------------------------------------------------------
