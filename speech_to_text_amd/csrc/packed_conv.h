@@ -181,7 +181,7 @@ struct ConvBwd {
 template <typename T, int K, int VEC>
 __global__ __launch_bounds__(256) void k_conv_bwd(const ConvBwd a) {
     using M = typename T::mem;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);       // row addresses in scalar registers
     const int cv = blockIdx.x * 64 + lane;
     const int c0 = cv * VEC;
     const bool live = cv < a.n_vec;
@@ -220,8 +220,8 @@ __global__ __launch_bounds__(256) void k_conv_bwd(const ConvBwd a) {
 #pragma unroll
             for (int g = 0; g < GROUP; ++g) { line[K - 1 + g] = next_x[g]; dyr[g] = next_dy[g]; }
             if (r + GROUP < r1 + (K - 1)) fetch(r + GROUP);
-            // the whole group, and the rows whose dx it completes, inside one sequence and this tile
-            const bool plain = q.inside && r - (K - 1) >= q.start && r - (K - 1) >= r0 && r + GROUP <= min(q.end, r1);
+            // the whole group, and the rows whose dx it completes, inside one sequence
+            const bool plain = q.inside && r - (K - 1) >= q.start && r + GROUP <= q.end;
 #pragma unroll
             for (int g = 0; g < GROUP; ++g) {
                 const int64_t row = r + g;
@@ -251,7 +251,7 @@ __global__ __launch_bounds__(256) void k_conv_bwd(const ConvBwd a) {
                             d[i] *= sg * fmaf(p, 1.0f - sg, 1.0f);
                         }
                     }
-                    if (plain || row < r1) {
+                    if (row < r1) {
 #pragma unroll
                         for (int i = 0; i < VEC; ++i) {
                             db[i] += d[i];
@@ -273,7 +273,7 @@ __global__ __launch_bounds__(256) void k_conv_bwd(const ConvBwd a) {
                     for (int j = 0; j < K; ++j)
 #pragma unroll
                         for (int i = 0; i < VEC; ++i) acc[i] = fmaf(w[K - 1 - j][i], dp[g + j][i], acc[i]);
-                    store_vec<M, VEC>(dx + o * a.dx_stride, acc, n);
+                    if (o >= r0 && o < r1) store_vec<M, VEC>(dx + o * a.dx_stride, acc, n);
                 } else if (o >= r0 && o < r1) {
                     const Place p = find_row(a.off, a.n_seqs, a.rows, o);
                     if (p.inside) {
@@ -320,32 +320,11 @@ __global__ __launch_bounds__(256) void k_conv_bwd(const ConvBwd a) {
     }
 }
 
-// dweight (channels, K) and dbias (channels) from the partial sums.
-template <typename T>
-__global__ __launch_bounds__(1024) void k_conv_sum(const float* __restrict__ part, int64_t n_part, int K, int channels,
-                                                   float* __restrict__ dweight, float* __restrict__ dbias) {
-    __shared__ float sh[16][64];
-    const int lane = threadIdx.x & 63, slice = threadIdx.x >> 6;
-    const int64_t m = (int64_t)(K + 1) * channels;
-    const int64_t e = (int64_t)blockIdx.x * 64 + lane;
-    sh[slice][lane] = e < m ? sum_strided(part + e, slice, 16, n_part, m) : 0.0f;
-    __syncthreads();
-    if (slice == 0 && e < m) {
-        float v = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v += sh[i][lane];
-        const int j = (int)(e / channels), c = (int)(e % channels);
-        if (j < K) dweight[(int64_t)c * K + j] = v;
-        else if (dbias) dbias[c] = v;
-    }
-}
-
 // Gradient of the initial state: row i of it lies K - 1 - i rows before the sequence and is read by the
 // rows q <= i with tap i - q; what a short sequence hands on of it comes back from dstate.
 template <typename T, int K>
-__global__ __launch_bounds__(256) void k_conv_dinitial(const ConvBwd a) {
+__device__ __forceinline__ void conv_dinitial(const ConvBwd& a, int64_t id) {
     using M = typename T::mem;
-    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (id >= (int64_t)a.n_seqs * a.channels) return;
     const int64_t s = id / a.channels;
     const int c = (int)(id % a.channels);
@@ -385,6 +364,31 @@ __global__ __launch_bounds__(256) void k_conv_dinitial(const ConvBwd a) {
         float v = di[i];
         if (dstate && i >= len) v += widen(dstate[(s * (K - 1) + i - len) * a.channels + c]);
         out[(s * (K - 1) + i) * a.channels + c] = narrow<M>(v);
+    }
+}
+
+// dweight (channels, K) and dbias (channels) from the partial sums; the blocks from `sum_blocks` on, if any, take
+// the gradient of the initial state.
+template <typename T, int K>
+__global__ __launch_bounds__(1024) void k_conv_finish(const ConvBwd a, int64_t n_part, int sum_blocks,
+                                                      float* __restrict__ dweight, float* __restrict__ dbias) {
+    __shared__ float sh[16][64];
+    if (blockIdx.x >= (unsigned)sum_blocks) {
+        conv_dinitial<T, K>(a, (int64_t)(blockIdx.x - sum_blocks) * 1024 + threadIdx.x);
+        return;
+    }
+    const int lane = threadIdx.x & 63, slice = threadIdx.x >> 6;
+    const int64_t m = (int64_t)(K + 1) * a.channels;
+    const int64_t e = (int64_t)blockIdx.x * 64 + lane;
+    sh[slice][lane] = e < m ? sum_strided(a.part + e, slice, 16, n_part, m) : 0.0f;
+    __syncthreads();
+    if (slice == 0 && e < m) {
+        float v = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v += sh[i][lane];
+        const int j = (int)(e / a.channels), c = (int)(e % a.channels);
+        if (j < K) dweight[(int64_t)c * K + j] = v;
+        else if (dbias) dbias[c] = v;
     }
 }
 
@@ -538,14 +542,12 @@ int conv_backward(const mfcc_conv_args* a, hipStream_t st) {
                                dim3(256), 0, st, f);
             PACKED_LAUNCHED();
         }
-        hipLaunchKernelGGL(k_conv_sum<T>, dim3((unsigned)ceil_div((int64_t)(K + 1) * a->channels, 64)), dim3(1024), 0, st,
-                           f.part, parts, K, a->channels, a->d_dweight, a->d_dbias);
+        const int64_t sum_blocks = ceil_div((int64_t)(K + 1) * a->channels, 64);
+        const int64_t more = a->d_dinitial && K > 1 ? ceil_div((int64_t)a->n_seqs * a->channels, 1024) : 0;
+        if (sum_blocks + more > 0x1fffff) return mfcc_detail::fail(MFCC_E_UNSUPPORTED, "batch too large: split it");
+        hipLaunchKernelGGL((k_conv_finish<T, K>), dim3((unsigned)(sum_blocks + more)), dim3(1024), 0, st, f, parts,
+                           (int)sum_blocks, a->d_dweight, a->d_dbias);
         PACKED_LAUNCHED();
-        if (a->d_dinitial && a->n_seqs > 0 && K > 1) {
-            hipLaunchKernelGGL((k_conv_dinitial<T, K>), dim3((unsigned)ceil_div((int64_t)a->n_seqs * a->channels, 256)),
-                               dim3(256), 0, st, f);
-            PACKED_LAUNCHED();
-        }
         return (int)MFCC_OK;
     });
 }
