@@ -367,7 +367,7 @@ int norm_forward(const mfcc_norm_args* a, hipStream_t st) {
     return by_width_of_row(f.width, [&](auto tpu, auto it) {
         constexpr int TPU = decltype(tpu)::value, IT = decltype(it)::value, PER = norm_block(TPU) / TPU;
         const int64_t blocks = ceil_div(f.rows * f.groups, PER);
-        if (blocks > 0x3fffff) return mfcc_detail::fail(MFCC_E_UNSUPPORTED, "batch too large: split it");
+        if (blocks * norm_block(TPU) > 0xffffffffll) return mfcc_detail::fail(MFCC_E_UNSUPPORTED, "batch too large: split it");
         hipLaunchKernelGGL((k_norm_fwd<T, RT, GATE, TPU, IT>), dim3((unsigned)blocks), dim3(norm_block(TPU)), 0, st, f);
         PACKED_LAUNCHED();
         return (int)MFCC_OK;

@@ -18,6 +18,8 @@ namespace packed {
 
 constexpr float SCAN_LOG2E = LOG2E;
 constexpr int SCAN_TILE = 32;       // rows of B and C staged in LDS at a time (forward kernels)
+constexpr int ZERO_ROW = SCAN_TILE;  // behind them one of zeros, for the missing rows of a group of four: with a step
+                                     // of zero as well they change nothing, also behind an infinite row
 
 // Holds the LDS reads of the next row back until half of this row's states are done: hoisted by the compiler,
 // the B and C of four rows take the registers of two wavefronts.
@@ -114,6 +116,7 @@ __device__ __forceinline__ void stage_rows(float* lds, const M* __restrict__ src
         const int n = i % NP;
         lds[i] = n < state ? widen(src[(row + i / NP) * stride + n]) : 0.0f;
     }
+    for (int n = threadIdx.x; n < NP; n += blockDim.x) lds[ZERO_ROW * NP + n] = 0.0f;
 }
 
 // A channel's states from n0 on in an (sequence, channel, n) array; zeros without the array.  Rarely run inside the
@@ -154,7 +157,7 @@ __device__ __forceinline__ void load_rates(float (&A2)[NP], const Scan& a, int c
 template <typename T, int NP, bool BACK>
 __global__ __launch_bounds__(256) void k_scan_sum(const Scan a) {
     using M = typename T::mem;
-    __shared__ float sB[SCAN_TILE * NP], sC[BACK ? SCAN_TILE * NP : 1];
+    __shared__ float sB[(SCAN_TILE + 1) * NP], sC[BACK ? (SCAN_TILE + 1) * NP : 1];
     const int slices = (a.state + NP - 1) / NP, n_blocks = a.groups * a.blocks_per_group * slices;
     const int sb = blockIdx.x % n_blocks, k = blockIdx.x / n_blocks;
     const int cb = sb / slices, n0 = sb % slices * NP;
@@ -225,7 +228,7 @@ __global__ __launch_bounds__(256) void k_scan_sum(const Scan a) {
                         float b[NP], cc[OPEN ? NP : 4];
                         row_of<NP>(b, sB + at);
                         if (OPEN) row_of<NP>(cc, sC + at);
-                        at += j + 1 < count ? NP : 0;
+                        at = j + 1 < count ? at + NP : ZERO_ROW * NP;
 #pragma unroll
                         for (int n = 0; n < NP; ++n) {
                             const float e = exp2_hw(d[j] * A2[n]);
@@ -324,7 +327,7 @@ __global__ __launch_bounds__(1024) void k_scan_carry(const Scan a) {
 template <typename T, int NP>
 __global__ __launch_bounds__(256) void k_scan_fwd(const Scan a) {
     using M = typename T::mem;
-    __shared__ float sB[SCAN_TILE * NP], sC[SCAN_TILE * NP];
+    __shared__ float sB[(SCAN_TILE + 1) * NP], sC[(SCAN_TILE + 1) * NP];
     const int n_blocks = a.groups * a.blocks_per_group;
     const int cb = blockIdx.x % n_blocks, k = blockIdx.x / n_blocks;
     const int g = cb / a.blocks_per_group;
@@ -397,7 +400,7 @@ __global__ __launch_bounds__(256) void k_scan_fwd(const Scan a) {
                     float b[NP], cc[NP];
                     row_of<NP>(b, sB + at);
                     row_of<NP>(cc, sC + at);
-                    at += j + 1 < count ? NP : 0;
+                    at = j + 1 < count ? at + NP : ZERO_ROW * NP;
 #pragma unroll
                     for (int n = 0; n < NP; ++n) {
                         h[n] = fmaf(exp2_hw(d[j] * A2[n]), h[n], du[j] * b[n]);

@@ -143,6 +143,11 @@ def _overlap(a, b) -> bool:
     return True
 
 
+def _flat(t):
+    """A contiguous state as rows, for the overlap check."""
+    return None if t is None else t.reshape(1, -1)
+
+
 def _out(out, x, inputs, dtype=None):
     """The output rows: new ones, or the caller's after a check."""
     if out is None:
@@ -218,6 +223,9 @@ def _differentiable(out, *tensors) -> bool:
 
 def _incoming(d, like):
     """A gradient from autograd as rows (an expanded one has no unit stride)."""
+    if torch.cuda.is_current_stream_capturing():
+        raise ParameterError("a differentiable call's backward pass cannot be captured into a graph: capture the "
+                             "*_backward function under torch.no_grad()")
     if d is None:
         return torch.zeros(like.shape, dtype=like.dtype, device=like.device)
     return d if d.stride(1) == 1 or d.shape[1] == 1 else d.contiguous()
@@ -245,7 +253,7 @@ def _conv_args(x, weight, bias, frame_offsets, activation, initial_state):
 
 def _conv_forward(x, weight, bias, frame_offsets, activation, initial_state, return_state, out):
     a, x, keep, n_seqs, width = _conv_args(x, weight, bias, frame_offsets, activation, initial_state)
-    y = _out(out, x, (x,))
+    y = _out(out, x, (x, _flat(initial_state)) if out is not None else ())
     a.d_y, a.y_stride, a.zero_rest = y.data_ptr(), y.stride(0), out is None
     state = None
     if return_state:
@@ -352,7 +360,7 @@ def causal_conv_step(x, state, weight, bias=None, *, activation=None, slots=None
     state = _state(state, "state", (n_slots, width - 1, channels), x.dtype, x, writable=True)
     new_state = _next_state(state, _state(new_state, "new_state", (n_slots, width - 1, channels), x.dtype, x, writable=True))
     slots = _slots(slots, batch, x)
-    y = _out(out, x, (x,))
+    y = _out(out, x, (x, _flat(state), _flat(new_state)) if out is not None else ())
     _run(x, _lib.lib().mfcc_causal_conv_step, _DTYPE[x.dtype], batch, n_slots, channels, width, _ACTIVATION[activation],
          x.data_ptr(), x.stride(0), state.data_ptr(), new_state.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(slots),
          y.data_ptr(), y.stride(0))
@@ -401,7 +409,7 @@ def _scan_forward(u, delta, A, B, Cm, D, delta_bias, frame_offsets, softplus, in
     shape = (n_seqs, u.shape[1], state)
     initial_state = _state(initial_state, "initial_state", shape, torch.float32, u)
     a.d_initial = _ptr(initial_state)
-    y = _out(out, u, (u, delta, B.flatten(1), Cm.flatten(1)) if out is not None else ())
+    y = _out(out, u, (u, delta, B.flatten(1), Cm.flatten(1), _flat(initial_state)) if out is not None else ())
     a.d_y, a.y_stride, a.zero_rest = y.data_ptr(), y.stride(0), out is None
     final = None
     if return_state:
@@ -488,7 +496,7 @@ def selective_scan_step(u, delta, A, B, C, state, D=None, delta_bias=None, *, so
     state = _state(state, "state", shape, torch.float32, u, writable=True)
     new_state = _next_state(state, _state(new_state, "new_state", shape, torch.float32, u, writable=True))
     slots = _slots(slots, u.shape[0], u)
-    y = _out(out, u, (u, delta, B.flatten(1), C.flatten(1)) if out is not None else ())
+    y = _out(out, u, (u, delta, B.flatten(1), C.flatten(1), _flat(state), _flat(new_state)) if out is not None else ())
     a.d_initial, a.d_final = state.data_ptr(), new_state.data_ptr()
     a.d_y, a.y_stride = y.data_ptr(), y.stride(0)
     _run(u, _lib.lib().mfcc_selective_scan_step, a, n_slots, _ptr(slots))

@@ -357,6 +357,31 @@ def test_scan_extreme_steps(gpu):
         assert abs(float(d[0, 0]) - want) <= 6 * 2.0 ** -24 * want + 2.0 ** -126, x
 
 
+def test_infinite_rows_stay_in_their_sequence(gpu):
+    """An infinite B, a NaN in u: the rows before them, and the other sequences with their gradients, do not see it."""
+    import speech_to_text_amd as S
+
+    g = gen(gpu, 63)
+    rows, ch, n = 90, 20, 16
+    off = [0, 38, 39, 83]
+    u, delta, A = rand(g, rows, ch, lo=0.5, hi=1.0), rand(g, rows, ch, lo=0.1, hi=0.2), -rand(g, ch, n, lo=0.1)
+    B, C, dy = randn(g, rows, n), randn(g, rows, n), randn(g, rows, ch)
+    want, state = S.selective_scan(u, delta, A, B, C, None, None, off, return_state=True)
+    grads = S.selective_scan_backward(dy, u, delta, A, B, C, None, None, off)
+    B2 = B.clone()
+    B2[37] = float("inf")                                   # the last row of the first sequence
+    y, s2 = S.selective_scan(u, delta, A, B2, C, None, None, off, return_state=True)
+    assert torch.equal(y[:37], want[:37]) and torch.equal(y[38:], want[38:])
+    assert torch.equal(s2[1:], state[1:]) and (s2[0] == float("inf")).all()
+    u2 = u.clone()
+    u2[38] = float("nan")                                   # a sequence of one row
+    y, s2 = S.selective_scan(u2, delta, A, B2, C, None, None, off, return_state=True)
+    assert torch.equal(y[:37], want[:37]) and torch.equal(y[39:], want[39:]) and torch.equal(s2[2], state[2])
+    g2 = S.selective_scan_backward(dy, u2, delta, A, B2, C, None, None, off)
+    for a, b in ((g2.u, grads.u), (g2.delta, grads.delta), (g2.B, grads.B), (g2.C, grads.C)):
+        assert torch.equal(a[39:], b[39:])
+
+
 # ---- norms ---------------------------------------------------------------------------------------------------------
 NORMS = [(1, 1), (3, 7), (9, 64), (5, 513), (2, 1000), (70, 96), (4, 2049), (3, 4100), (2, 9001), (1, 20000), (300, 40),
          (6, 1500), (77, 200), (3, 7000),
@@ -1011,6 +1036,10 @@ def test_refusals(gpu):
     state = torch.zeros(11, 3, 6, device=gpu)
     with pytest.raises(S.ParameterError):
         S.causal_conv_step(x, state[:10], w, new_state=state[1:])
+    with pytest.raises(S.ParameterError):                    # the result in the middle of the states
+        S.causal_conv_step(x, state[:10], w, out=state.view(33, 6)[:10])
+    with pytest.raises(S.ParameterError):
+        S.causal_conv(x, w, None, [0, 10], initial_state=state[:1], out=state.view(33, 6)[:10])
 
 
 def test_differentiable_calls_are_not_captured(gpu):
