@@ -268,8 +268,8 @@ __global__ __launch_bounds__(256) void k_scan_sum(const Scan a) {
 
 // Pass 2, in place: hst[k] (and, from the right, gst[k]) becomes the state that enters chunk k.  64 columns
 // by 16 segments of the chunks: each segment's own composition, then the ones before it, then the segment.
-// Sixteen chunks are loaded at a time: one after the other they are a chain of memory latencies.
-template <typename T>
+// BATCH chunks are loaded at a time: one after the other they are a chain of memory latencies.
+template <typename T, int BATCH>
 __global__ __launch_bounds__(1024) void k_scan_carry(const Scan a) {
     __shared__ float sD[16][64], sH[16][64];
     const int lane = threadIdx.x & 63, seg = threadIdx.x >> 6;
@@ -282,7 +282,6 @@ __global__ __launch_bounds__(1024) void k_scan_carry(const Scan a) {
     const float A2 = a.A[(int64_t)c * a.state + n] * SCAN_LOG2E;
     const int len = (a.n_chunks + 15) / 16;
     const int k0 = min(seg * len, a.n_chunks), k1 = min(k0 + len, a.n_chunks);
-    constexpr int BATCH = 16;
     float v[BATCH], dec[BATCH];
     int cut[BATCH];
     auto fetch = [&](int i0) {
@@ -476,12 +475,12 @@ __device__ __forceinline__ float sum_channels(float v) {     // over the lanes o
 // Eight neighbouring elements in LDS, 16 bytes aligned.
 template <typename M> struct alignas(16) Eight { Raw<M, SUB> r; };
 
-template <typename T, int NP>
+template <typename T, int NP, int MAXR>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(bwd_waves<T, NP>()))) void k_scan_bwd(const Scan a) {
     using M = typename T::mem;
-    constexpr int LPC = bwd_lpc<NP>(), CPW = WAVE / LPC, CPB = 4 * CPW, MAXR = bwd_rows<NP>(), NSUB = MAXR / SUB;
+    constexpr int LPC = bwd_lpc<NP>(), CPW = WAVE / LPC, CPB = 4 * CPW, NSUB = MAXR / SUB;
     constexpr int SD = MAXR + 4, SM = MAXR + 16 / (int)sizeof(M);      // distance between channels
-    constexpr int QUADS = CPB / 4, PASS_ROWS = 256 / QUADS, PASSES = MAXR / PASS_ROWS;   // staging: four channels a thread
+    constexpr int QUADS = CPB / 4, PASS_ROWS = 256 / QUADS, PASSES = (MAXR + PASS_ROWS - 1) / PASS_ROWS;   // staging: four channels a thread
     __shared__ alignas(16) float sd[CPB * SD];           // d, later the gradient of d
     __shared__ alignas(16) M su[CPB * SM];               // u, later its gradient
     __shared__ alignas(16) M sdy[CPB * SM];
@@ -551,9 +550,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(bwd_waves<T
                 const float d = has ? step_of(a.softplus, narrow<M>(raw[p][i]), bias[i]) : 0.0f;
                 const float x = has ? uv[p][i] : 0.0f, y = has ? dv[p][i] : 0.0f;
                 dD[i] = fmaf(x, y, dD[i]);
-                sd[(sq + i) * SD + t] = d;
-                su[(sq + i) * SM + t] = narrow<M>(x);
-                sdy[(sq + i) * SM + t] = narrow<M>(y);
+                if (t < MAXR) {
+                    sd[(sq + i) * SD + t] = d;
+                    su[(sq + i) * SM + t] = narrow<M>(x);
+                    sdy[(sq + i) * SM + t] = narrow<M>(y);
+                }
             }
         }
         fold(dD, a.part_D);
@@ -992,6 +993,13 @@ int scan_empties(const mfcc_scan_args* a, const float* from, float* to, hipStrea
 }
 
 template <typename T>
+void launch_carry(const Scan& f, unsigned directions, hipStream_t st) {
+    const dim3 grid((unsigned)ceil_div((int64_t)f.state * f.channels, 64), directions);
+    if (f.n_chunks <= 16 * 8) hipLaunchKernelGGL((k_scan_carry<T, 8>), grid, dim3(1024), 0, st, f);
+    else hipLaunchKernelGGL((k_scan_carry<T, 16>), grid, dim3(1024), 0, st, f);
+}
+
+template <typename T>
 int scan_forward(const mfcc_scan_args* a, hipStream_t st) {
     Scan f = scan_args(a, false);
     const int block = scan_block(f.per);
@@ -1005,8 +1013,7 @@ int scan_forward(const mfcc_scan_args* a, hipStream_t st) {
                 if (grid * sum_slices(f.state, false) > 0x7fffff) return mfcc_detail::fail(MFCC_E_UNSUPPORTED, "batch too large: split it");
                 hipLaunchKernelGGL((k_scan_sum<T, std::min(NP, sum_states(false)), false>), dim3((unsigned)(grid * sum_slices(f.state, false))),
                                    dim3(block), 0, st, f);
-                hipLaunchKernelGGL(k_scan_carry<T>, dim3((unsigned)ceil_div((int64_t)f.state * f.channels, 64), 1), dim3(1024),
-                                   0, st, f);
+                launch_carry<T>(f, 1, st);
             }
             hipLaunchKernelGGL((k_scan_fwd<T, NP>), dim3((unsigned)grid), dim3(block), 0, st, f);
             PACKED_LAUNCHED();
@@ -1031,13 +1038,14 @@ int scan_backward(const mfcc_scan_args* a, hipStream_t st) {
                 if (grid * sum_slices(f.state, true) > 0x7fffff) return mfcc_detail::fail(MFCC_E_UNSUPPORTED, "batch too large: split it");
                 hipLaunchKernelGGL((k_scan_sum<T, std::min(NP, sum_states(true)), true>), dim3((unsigned)(grid * sum_slices(f.state, true))),
                                    dim3(block), 0, st, f);
-                hipLaunchKernelGGL(k_scan_carry<T>, dim3((unsigned)ceil_div((int64_t)f.state * f.channels, 64), 2), dim3(1024),
-                                   0, st, f);
+                launch_carry<T>(f, 2, st);
             }
             f.blocks_per_group = (int)ceil_div(f.per, bwd_channels<NP>());
             const int64_t grid2 = (int64_t)f.groups * f.blocks_per_group * f.n_chunks;
             if (grid2 > 0x7fffff) return mfcc_detail::fail(MFCC_E_UNSUPPORTED, "batch too large: split it");
-            hipLaunchKernelGGL((k_scan_bwd<T, NP>), dim3((unsigned)grid2), dim3(256), 0, st, f);
+            // chunks of up to sixteen rows in a kernel with LDS for as many: three times the workgroups per CU
+            if (f.chunk <= 16) hipLaunchKernelGGL((k_scan_bwd<T, NP, 16>), dim3((unsigned)grid2), dim3(256), 0, st, f);
+            else hipLaunchKernelGGL((k_scan_bwd<T, NP, bwd_rows<NP>()>), dim3((unsigned)grid2), dim3(256), 0, st, f);
             PACKED_LAUNCHED();
         }
         const int64_t m = a->rows * f.groups * NP;
