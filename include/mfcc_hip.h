@@ -251,6 +251,7 @@ int mfcc_delta(const float* d_feats, const int64_t* d_frame_offsets, const int64
  *   - activations are MFCC_F32, MFCC_BF16 or MFCC_F16; learned tables, their gradients and the
  *     scan's states are float32; all arithmetic is float32, rounded once into the output;
  *   - sums run in a fixed order: the same call gives the same bits;
+ *   - outputs overlap no input and no other output, except where it says so;
  *   - everything is asynchronous on `stream`, allocates nothing and can be captured; workspaces are
  *     256-byte aligned, needed until the call's work is done, and not shared by calls that may overlap. */
 enum { MFCC_F32 = 0, MFCC_BF16 = 1, MFCC_F16 = 2 };

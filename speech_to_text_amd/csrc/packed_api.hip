@@ -166,7 +166,7 @@ int mfcc_gate_norm(const mfcc_norm_args* a, void* stream) try {
 
 size_t mfcc_norm_backward_workspace(const mfcc_norm_args* a) {
     if (check_norm(a, true) && check_norm(a, false)) return 0;
-    return (size_t)norm_bwd_blocks(a) * 3 * (size_t)a->channels * sizeof(float);
+    return norm_bwd_space(a);
 }
 
 int mfcc_add_norm_backward(const mfcc_norm_args* a, void* stream) try {

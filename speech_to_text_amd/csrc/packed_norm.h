@@ -4,7 +4,8 @@
 //   norm:  v / sqrt(mean(v^2) + eps), of v - mean(v) for the layer form.
 // Bound by memory: every row is read once, held in registers (eight neighbouring elements a thread and
 // step), reduced over 16 to 1024 threads and written once.  The layer form's deviation is summed
-// around the mean, from the registers.
+// around the mean, from the registers.  16384 x 2048, bfloat16 with a float32 residual: 82 us forward (4.9 TB/s), 120 us
+// backward (5.0 TB/s); the gate over 30011 x 4096 in 8 groups, bfloat16: 134 us (5.5 TB/s).
 #pragma once
 #include "packed.h"
 
@@ -21,6 +22,7 @@ struct Norm {
     const float *weight, *bias, *scale;
     void *y, *r, *dx, *dz, *dresidual;
     float* part;               // (blocks, 3, channels): dweight, dbias, dscale
+    float4* stats;             // wide rows: mean, 1 / deviation, and their gradient's (rows, groups)
     int64_t rows;
     int channels, groups, width, layer, gate_first;
     float eps, scale_value, inv_width;
@@ -305,6 +307,140 @@ __global__ __launch_bounds__(norm_block(TPU)) void k_norm_bwd(const Norm a) {
     }
 }
 
+// ---- gradients of wide rows ----------------------------------------------------------------------------
+// A row wider than the registers of a workgroup hold is read twice (three times for the layer form, whose deviation
+// is summed around the mean), the second time from a cache.  The sums over rows are left to k_norm_columns, which
+// reads everything once more with a thread per eight columns and takes the row's statistics from the workspace.
+// Bound by memory: 1000 x 32768 in 122 us in bfloat16, 250 us in float32 (2.1 TB/s of the four tensors, each read twice).
+
+// Eight columns of a row.
+template <typename T, typename RT, bool GATE>
+struct NormColumns {
+    float dy[NV], x[NV], z[NV], r[NV], dr[NV], w[NV], t[NV];
+    __device__ __forceinline__ void tables(const Norm& a, int c, int n) {
+        load_or<float>(w, a.weight ? a.weight + c : nullptr, n, 1.0f);
+        if (GATE) load_or<float>(t, a.bias ? a.bias + c : nullptr, n, 0.0f);
+        else load_or<float>(t, a.scale ? a.scale + c : nullptr, n, a.scale_value);
+    }
+    __device__ __forceinline__ void row(const Norm& a, int64_t row, int c, int n, bool all) {
+        using M = typename T::mem;
+        using RM = typename RT::mem;
+        load_or<M>(dy, a.dy ? static_cast<const M*>(a.dy) + row * a.dy_stride + c : nullptr, n, 0.0f);
+        if (GATE) {
+            load_vec<M, NV>(x, static_cast<const M*>(a.x) + row * a.x_stride + c, n);
+            load_vec<M, NV>(z, static_cast<const M*>(a.z) + row * a.z_stride + c, n);
+        } else {
+            load_vec<RM, NV>(r, static_cast<const RM*>(a.r_in) + row * a.r_stride + c, n);
+            if (!all) return;
+            load_or<RM>(dr, a.dr ? static_cast<const RM*>(a.dr) + row * a.dr_stride + c : nullptr, n, 0.0f);
+            load_or<M>(x, a.x ? static_cast<const M*>(a.x) + row * a.x_stride + c : nullptr, n, 0.0f);
+        }
+    }
+    __device__ __forceinline__ float gate(int i) const { return z[i] * sigmoid_f<sizeof(typename T::mem) == 4>(z[i]); }
+    // the value that is normalised, and the gradient of the normalised one
+    __device__ __forceinline__ float value(const Norm& a, int i) const { return !GATE ? r[i] : a.gate_first ? x[i] * gate(i) : x[i]; }
+    __device__ __forceinline__ float grad(const Norm& a, int i) const {
+        return (GATE && !a.gate_first ? dy[i] * gate(i) : dy[i]) * w[i];
+    }
+};
+
+template <typename T, typename RT, bool GATE>
+__global__ __launch_bounds__(1024) void k_norm_bwd_wide(const Norm a) {
+    using M = typename T::mem;
+    using RM = typename RT::mem;
+    __shared__ float sh[16][2];
+    for (int64_t unit = blockIdx.x; unit < a.rows * a.groups; unit += gridDim.x) {
+        const int64_t row = unit / a.groups;
+        const int c_base = (int)(unit % a.groups) * a.width;
+        NormColumns<T, RT, GATE> in;
+        float mean = 0.0f, dmean = 0.0f, s = 0.0f, t = 0.0f;
+        if (a.layer) {
+            for (int w0 = threadIdx.x * NV; w0 < a.width; w0 += 1024 * NV) {
+                const int n = a.width - w0;
+                in.tables(a, c_base + w0, n);
+                in.row(a, row, c_base + w0, n, false);
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+                    if (i < n) { s += in.value(a, i); t += in.grad(a, i); }
+            }
+            unit_sum2<1024>(s, t, sh);
+            mean = s * a.inv_width; dmean = t * a.inv_width;
+            s = t = 0.0f;
+        }
+        for (int w0 = threadIdx.x * NV; w0 < a.width; w0 += 1024 * NV) {
+            const int n = a.width - w0;
+            in.tables(a, c_base + w0, n);
+            in.row(a, row, c_base + w0, n, false);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const float d = i < n ? in.value(a, i) - mean : 0.0f;
+                s = fmaf(d, d, s);
+                if (i < n) t = fmaf(in.grad(a, i), d, t);
+            }
+        }
+        unit_sum2<1024>(s, t, sh);
+        const float q = rsqrtf(fmaf(s, a.inv_width, a.eps)), proj = t * a.inv_width * q;
+        if (a.part && threadIdx.x == 0) a.stats[unit] = make_float4(mean, q, dmean, proj);
+        for (int w0 = threadIdx.x * NV; w0 < a.width; w0 += 1024 * NV) {
+            const int c = c_base + w0, n = a.width - w0;
+            const int64_t at = row * a.channels + c;
+            in.tables(a, c, n);
+            in.row(a, row, c, n, true);
+            float dv[NV], dz[NV];
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const float vn = (in.value(a, i) - mean) * q;
+                dv[i] = (in.grad(a, i) - dmean - vn * proj) * q;
+                if (GATE) {
+                    const float z = in.z[i], sg = sigmoid_f<sizeof(M) == 4>(z), slope = sg * fmaf(z, 1.0f - sg, 1.0f);
+                    dz[i] = (a.gate_first ? dv[i] * in.x[i] : in.dy[i] * fmaf(vn, in.w[i], in.t[i])) * slope;
+                    if (a.gate_first) dv[i] *= z * sg;
+                } else {
+                    dv[i] += in.dr[i];
+                }
+            }
+            if (GATE) {
+                store_vec<M, NV>(static_cast<M*>(a.dx) + at, dv, n);
+                store_vec<M, NV>(static_cast<M*>(a.dz) + at, dz, n);
+            } else {
+                if (a.dresidual) store_vec<RM, NV>(static_cast<RM*>(a.dresidual) + at, dv, n);
+                if (a.dx) {
+#pragma unroll
+                    for (int i = 0; i < NV; ++i) dv[i] *= in.t[i];
+                    store_vec<M, NV>(static_cast<M*>(a.dx) + at, dv, n);
+                }
+            }
+        }
+    }
+}
+
+template <typename T, typename RT, bool GATE>
+__global__ __launch_bounds__(256) void k_norm_columns(const Norm a) {
+    const int g = blockIdx.y, w0 = (blockIdx.z * 256 + threadIdx.x) * NV, c = g * a.width + w0, n = a.width - w0;
+    if (n <= 0) return;
+    NormColumns<T, RT, GATE> in;
+    in.tables(a, c, n);
+    float sum[GATE ? 2 : 3][NV] = {};
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const float4 st = a.stats[row * a.groups + g];           // mean, q, dmean, proj
+        in.row(a, row, c, n, true);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const float vn = (in.value(a, i) - st.x) * st.y;
+            const float body = GATE && !a.gate_first ? in.dy[i] * in.gate(i) : in.dy[i];
+            sum[0][i] = fmaf(body, vn, sum[0][i]);
+            sum[1][i] += body;
+            if (!GATE) {
+                const float dv = fmaf(in.grad(a, i) - st.z - vn * st.w, st.y, in.dr[i]);
+                sum[GATE ? 0 : 2][i] = fmaf(dv, in.x[i], sum[GATE ? 0 : 2][i]);
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < (GATE ? 2 : 3); ++j)
+        store_vec<float, NV>(a.part + ((int64_t)blockIdx.x * 3 + j) * a.channels + c, sum[j], n);
+}
+
 template <typename T>
 __global__ __launch_bounds__(1024) void k_norm_reduce(const float* __restrict__ part, int n_part, int channels, float* dweight,
                                                       float* dbias, float* dscale) {
@@ -327,7 +463,7 @@ __global__ __launch_bounds__(1024) void k_norm_reduce(const float* __restrict__ 
 constexpr int NORM_MAX_WIDTH = 32768;
 
 // Threads per row and steps of eight elements per thread: (16, 1) .. (1024, 4).
-template <typename Fn>
+template <int MOST, typename Fn>
 int by_width_of_row(int width, Fn&& fn) {
     using std::integral_constant;
     if (width <= 128) return fn(integral_constant<int, 16>{}, integral_constant<int, 1>{});
@@ -336,16 +472,28 @@ int by_width_of_row(int width, Fn&& fn) {
     if (width <= 1024) return fn(integral_constant<int, 128>{}, integral_constant<int, 1>{});
     if (width <= 2048) return fn(integral_constant<int, 256>{}, integral_constant<int, 1>{});
     if (width <= 4096) return fn(integral_constant<int, 256>{}, integral_constant<int, 2>{});
-    if (width <= 8192) return fn(integral_constant<int, 512>{}, integral_constant<int, 2>{});
-    if (width <= 16384) return fn(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
-    return fn(integral_constant<int, 1024>{}, integral_constant<int, 4>{});
+    if (MOST <= 8192 || width <= 8192) return fn(integral_constant<int, 512>{}, integral_constant<int, 2>{});
+    if constexpr (MOST > 8192) {
+        if (width <= 16384) return fn(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
+        return fn(integral_constant<int, 1024>{}, integral_constant<int, 4>{});
+    }
 }
 
-// Blocks that walk over the rows in the backward pass: about four wavefronts for each of the 1024 SIMDs.
+// Rows up to this width stay in registers in the gradients too (4000 x 8192 bfloat16: 72 us, against 130 us by
+// k_norm_bwd_wide); wider ones would spill (1000 x 20000: 368 us, against 83 us).
+constexpr int NORM_HELD = 8192;
+
+// Blocks that walk over the rows in the backward pass, each with a row of partial sums: about four wavefronts for
+// each of the 1024 SIMDs.
 inline int norm_bwd_blocks(const mfcc_norm_args* a) {
     const int width = a->channels / a->groups, per = width <= 128 ? 16 : width <= 256 ? 8 : width <= 512 ? 4 : 1;
     const int64_t blocks = width <= 512 ? 1024 : width <= 1024 ? 2048 : width <= 4096 ? 1024 : 512;
-    return (int)std::min<int64_t>(ceil_div(a->rows, per), std::max<int64_t>(1, blocks / a->groups));
+    const int64_t tiles = width > NORM_HELD ? ceil_div(width, 256 * NV) : 1;
+    return (int)std::min<int64_t>(ceil_div(a->rows, per), std::max<int64_t>(1, (width > NORM_HELD ? 2048 : blocks) / (a->groups * tiles)));
+}
+inline size_t norm_bwd_space(const mfcc_norm_args* a) {
+    const size_t stats = a->channels / a->groups > NORM_HELD ? (size_t)a->rows * a->groups * sizeof(float4) : 0;
+    return stats + (size_t)norm_bwd_blocks(a) * 3 * (size_t)a->channels * sizeof(float);
 }
 
 inline Norm norm_args(const mfcc_norm_args* a) {
@@ -364,7 +512,7 @@ template <typename T, typename RT, bool GATE>
 int norm_forward(const mfcc_norm_args* a, hipStream_t st) {
     if (a->rows == 0) return MFCC_OK;
     const Norm f = norm_args(a);
-    return by_width_of_row(f.width, [&](auto tpu, auto it) {
+    return by_width_of_row<NORM_MAX_WIDTH>(f.width, [&](auto tpu, auto it) {
         constexpr int TPU = decltype(tpu)::value, IT = decltype(it)::value, PER = norm_block(TPU) / TPU;
         const int64_t blocks = ceil_div(f.rows * f.groups, PER);
         if (blocks * norm_block(TPU) > 0xffffffffll) return mfcc_detail::fail(MFCC_E_UNSUPPORTED, "batch too large: split it");
@@ -380,21 +528,34 @@ int norm_backward(const mfcc_norm_args* a, hipStream_t st) {
     if (!a->d_dscale && !GATE) f.x = nullptr;
     const int blocks = norm_bwd_blocks(a);
     const bool sums = a->d_dweight || a->d_dbias || a->d_dscale;
-    f.part = sums ? static_cast<float*>(a->d_workspace) : nullptr;
-    return by_width_of_row(f.width, [&](auto tpu, auto it) {
-        constexpr int TPU = decltype(tpu)::value, IT = decltype(it)::value;
-        if (blocks > 0) {
+    const bool wide = f.width > NORM_HELD;
+    if (sums) {
+        f.stats = static_cast<float4*>(a->d_workspace);
+        f.part = static_cast<float*>(a->d_workspace) + (wide ? f.rows * f.groups * 4 : 0);
+    }
+    if (blocks > 0 && wide) {
+        const unsigned tiles = (unsigned)ceil_div(f.width, 256 * NV);
+        const int64_t units = std::min<int64_t>(f.rows * f.groups, 1 << 16);
+        hipLaunchKernelGGL((k_norm_bwd_wide<T, RT, GATE>), dim3((unsigned)units), dim3(1024), 0, st, f);
+        if (sums)
+            hipLaunchKernelGGL((k_norm_columns<T, RT, GATE>), dim3((unsigned)blocks, (unsigned)f.groups, tiles), dim3(256), 0, st, f);
+        PACKED_LAUNCHED();
+    } else if (blocks > 0) {
+        const int rc = by_width_of_row<NORM_HELD>(f.width, [&](auto tpu, auto it) {
+            constexpr int TPU = decltype(tpu)::value, IT = decltype(it)::value;
             hipLaunchKernelGGL((k_norm_bwd<T, RT, GATE, TPU, IT>), dim3((unsigned)blocks, (unsigned)f.groups),
                                dim3(norm_block(TPU)), 0, st, f);
             PACKED_LAUNCHED();
-        }
-        if (sums) {
-            hipLaunchKernelGGL(k_norm_reduce<T>, dim3((unsigned)ceil_div(f.channels, 64), 3), dim3(1024), 0, st, f.part, blocks,
-                               f.channels, a->d_dweight, a->d_dbias, a->d_dscale);
-            PACKED_LAUNCHED();
-        }
-        return (int)MFCC_OK;
-    });
+            return (int)MFCC_OK;
+        });
+        if (rc) return rc;
+    }
+    if (sums) {
+        hipLaunchKernelGGL(k_norm_reduce<T>, dim3((unsigned)ceil_div(f.channels, 64), 3), dim3(1024), 0, st, f.part, blocks,
+                           f.channels, a->d_dweight, a->d_dbias, a->d_dscale);
+        PACKED_LAUNCHED();
+    }
+    return (int)MFCC_OK;
 }
 
 template <typename T>

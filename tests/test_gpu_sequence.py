@@ -386,7 +386,9 @@ def test_infinite_rows_stay_in_their_sequence(gpu):
 NORMS = [(1, 1), (3, 7), (9, 64), (5, 513), (2, 1000), (70, 96), (4, 2049), (3, 4100), (2, 9001), (1, 20000), (300, 40),
          (6, 1500), (77, 200), (3, 7000),
          # rows enough that a workgroup of the gradient kernels walks over several, for each number of threads per row
-         (20000, 24), (9000, 130), (4500, 300), (2500, 1100), (2300, 600)]
+         (20000, 24), (9000, 130), (4500, 300), (2500, 1100), (2300, 600),
+         # rows too wide for the registers: two groups, one, the widest
+         (450, 16390), (260, 8193), (2, 32768)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -483,6 +485,29 @@ def test_gate_norm(gpu, case, dtype):
     R.assert_close(got.weight, refs[2], F32, (body * n * (1 + n)).sum(0), rows + 2 * chain, "weight")
     if rb is not None:
         R.assert_close(got.bias, refs[3], F32, body.sum(0), rows + 12, "bias")
+
+
+def test_gradients_of_more_wide_rows_than_workgroups(gpu):
+    """Every row's gradient is the one it has in a batch of a few rows; the sum over rows holds against 64 bits."""
+    import speech_to_text_amd as S
+
+    rows, ch = 65536 + 70, 8193
+    g = torch.Generator(device=gpu).manual_seed(77)
+    x, z, dy = (torch.empty(rows, ch, dtype=BF16, device=gpu).normal_(generator=g) for _ in range(3))
+    w = torch.ones(ch, device=gpu)
+    got = S.gate_norm_backward(dy, x, z, w)
+    for part in (slice(0, 3), slice(40000, 40005), slice(65530, rows)):
+        few = S.gate_norm_backward(dy[part], x[part], z[part], w)
+        assert torch.equal(got.x[part], few.x) and torch.equal(got.z[part], few.z)
+    want, size = (torch.zeros(ch, dtype=torch.float64, device=gpu) for _ in range(2))
+    for i in range(0, rows, 4096):
+        p = slice(i, i + 4096)
+        n = dy[p].double() * R.norm(x[p].double() * R.silu(z[p].double()), "rms", 1e-5)
+        want += n.sum(0)
+        size += n.abs().sum(0)
+    # each value's own error (the gate's and the norm's, as in the smaller cases), and the sum: a chain of rows / workgroups
+    # (409, of five tiles in 2048) in each partial sum and of 16 slices over them
+    R.assert_close(got.weight, want.cpu(), F32, size.cpu(), rows / 409 + 409 / 16 + 20 + 2 * (ch / 64 + 34), "weight")
 
 
 def test_norms_of_special_rows(gpu):
