@@ -49,7 +49,7 @@ int fail(int code, const std::string& msg) {
 
 }  // namespace
 
-// The same convention for the other translation units (packed_*.hip).
+// The same convention for the other translation units (packed_api.hip, packed_inst.hip).
 namespace mfcc_detail {
 int fail(int code, const char* msg) {
     try { g_err = msg; } catch (...) {}

@@ -1,4 +1,4 @@
-// Shared by the operators over packed rows (packed_conv.hip, packed_scan.hip, packed_norm.hip):
+// Shared by the operators over packed rows (packed_conv.h, packed_scan.h, packed_norm.h):
 // element types, wide loads at any element alignment, the place of a row in its sequence, wavefront
 // sums, and the error convention of the C ABI.
 #pragma once

@@ -10,7 +10,9 @@
 // A chunk that holds the start of a sequence lets nothing through (its decay counts as zero).
 //
 // Bound by vector issue, not memory: per (row, channel, n) one exp (8 SIMD cycles per wavefront) and four to
-// five plain operations (2.6 each) per pass against 6 / N bytes in 16-bit types.
+// five plain operations (2.6 each) per pass against 6 / N bytes in 16-bit types.  16384 x 2048, 16 states, bfloat16:
+// 116 + 10 + 147 us for the three passes (the two sweeps 4.6 and 3.7 10^12 elements (row, channel, n) a second).
+// The first sweep is what the split costs; undivided, 2048 channels are 32 wavefronts for 1024 SIMDs.
 #pragma once
 #include "packed.h"
 
@@ -153,7 +155,8 @@ __device__ __forceinline__ void load_rates(float (&A2)[NP], const Scan& a, int c
 }
 
 // Pass 1.  A lane holds a channel and up to sixteen of its states (they are independent here: more of them are
-// more workgroups); B and C come from LDS.
+// more workgroups); B and C come from LDS.  With the reverse part a lane holds eight: its four tables of sixteen would
+// not fit the registers of four wavefronts per SIMD (12007 x 2048 x 16 in bfloat16: 137 us, 92 us without).
 template <typename T, int NP, bool BACK>
 __global__ __launch_bounds__(256) void k_scan_sum(const Scan a) {
     using M = typename T::mem;
@@ -268,7 +271,8 @@ __global__ __launch_bounds__(256) void k_scan_sum(const Scan a) {
 
 // Pass 2, in place: hst[k] (and, from the right, gst[k]) becomes the state that enters chunk k.  64 columns
 // by 16 segments of the chunks: each segment's own composition, then the ones before it, then the segment.
-// BATCH chunks are loaded at a time: one after the other they are a chain of memory latencies.
+// BATCH chunks are loaded at a time: one after the other they are a chain of memory latencies.  Bound by memory:
+// 128 chunks of 2048 x 16 states read and written in 10 us (3.3 TB/s).
 template <typename T, int BATCH>
 __global__ __launch_bounds__(1024) void k_scan_carry(const Scan a) {
     __shared__ float sD[16][64], sH[16][64];
@@ -322,7 +326,8 @@ __global__ __launch_bounds__(1024) void k_scan_carry(const Scan a) {
     }
 }
 
-// Pass 3: y, and the states that sequences leave behind.
+// Pass 3: y, and the states that sequences leave behind.  A lane holds a channel with all its states, so that the sum
+// over them needs no other lane.  Four rows of u and delta are in flight; 147 us at 16384 x 2048 x 16 in bfloat16.
 template <typename T, int NP>
 __global__ __launch_bounds__(256) void k_scan_fwd(const Scan a) {
     using M = typename T::mem;
@@ -444,6 +449,8 @@ __global__ __launch_bounds__(256) void k_scan_empty(const int64_t* __restrict__ 
 // latencies overlap.  Sums over n stay in the LPC lanes of a channel; dB and dC are summed over the channels of the
 // wavefront (v_permlane swaps halve eight values to two, then rotations within a row of lanes), over the four
 // wavefronts in LDS, and over the workgroups of a group by k_scan_reduce: a fixed order throughout.
+// Bound by vector issue: 113 instructions per wavefront and row (256 elements), two of eight an exp; the vector units
+// are busy 91 % of the time.  12007 x 2048 x 16 in bfloat16: 415 us.
 constexpr int SUB = 8;
 
 template <int NP> constexpr int bwd_lpc() { return NP / 4; }
@@ -759,7 +766,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(bwd_waves<T
 }
 
 // The sums of the partial results, one launch for all of them: out[e] = sum over parts of part[p][e], of rows of
-// `padded` columns of which the first `inner` are kept.  64 elements by 16 slices of the parts.
+// `padded` columns of which the first `inner` are kept.  64 elements by 16 slices of the parts.  17 us for the
+// 65 MB of 12007 x 2048 x 16.
 struct ReduceJob {
     const float* part; void* out;
     int64_t n_part, m, first_block;
@@ -809,7 +817,8 @@ struct ScanStep {
 // Entries that name the same slot are successive tokens of that sequence and are taken by the first of
 // them; a slot outside the pool gives a zero row and touches no state.  A thread has four states of a channel for
 // NE entries: their loads, which need the slots alone, go out together and before the list of slots is looked
-// through (a wavefront with one entry waits more than it moves: 3.2 TB/s), and A is read once for them.
+// through (a wavefront with one entry waits more than it moves: 3.2 TB/s), and A is read once for them
+// (256 x 4096 x 16: 32 us, 4.3 TB/s).
 template <typename T, int NP, int NE>
 __global__ __launch_bounds__(256) void k_scan_step(const ScanStep a) {
     using M = typename T::mem;
