@@ -230,18 +230,31 @@ __device__ __forceinline__ float lanes_sum(float v) {
     return v;
 }
 
-// Whether another entry of a batch names the slot of entry e0, before or after it.  Every wavefront looks
-// through the whole list by itself, 64 entries at a time.
-struct SlotUse { bool before, after; };
-__device__ __forceinline__ SlotUse slot_use(const int32_t* __restrict__ slots, int batch, int e0) {
-    const int slot = slots[e0];
-    bool before = false, after = false;
-    for (int e = threadIdx.x & 63; e < batch; e += WAVE) {
-        const bool same = slots[e] == slot;
-        before |= same && e < e0;
-        after |= same && e > e0;
+// Whether another entry of a batch names the slot of entry e0 + k, before or after it.  The four wavefronts of the
+// workgroup share the list; a short one each looks through by itself.
+template <int NE>
+__device__ __forceinline__ void slot_use(bool (&before)[NE], bool (&after)[NE], const int32_t* __restrict__ slots, int batch,
+                                         int e0, const int (&slot)[NE]) {
+    __shared__ unsigned found[4];
+    const bool alone = batch <= WAVE;
+    unsigned bits = 0;
+#pragma unroll 4
+    for (int e = alone ? threadIdx.x & 63 : threadIdx.x; e < batch; e += 256) {
+        const int other = slots[e];
+#pragma unroll
+        for (int k = 0; k < NE; ++k)
+            if (other == slot[k]) bits |= (e < e0 + k ? 1u : e > e0 + k ? 16u : 0u) << k;
     }
-    return {__ballot(before) != 0, __ballot(after) != 0};
+    unsigned all = 0;
+#pragma unroll
+    for (int k = 0; k < NE; ++k) all |= (__ballot(bits >> k & 1) ? 1u << k : 0u) | (__ballot(bits >> k & 16) ? 16u << k : 0u);
+    if (!alone) {
+        if ((threadIdx.x & 63) == 0) found[threadIdx.x >> 6] = all;
+        __syncthreads();
+        all = found[0] | found[1] | found[2] | found[3];
+    }
+#pragma unroll
+    for (int k = 0; k < NE; ++k) { before[k] = all >> k & 1; after[k] = all >> k & 16; }
 }
 
 // Workgroups are dealt to the eight XCDs in turn.  This gives each XCD a contiguous eighth of the work, so that

@@ -462,7 +462,9 @@ __global__ __launch_bounds__(1024) void k_norm_reduce(const float* __restrict__ 
 // ---- host --------------------------------------------------------------------------------------------
 constexpr int NORM_MAX_WIDTH = 32768;
 
-// Threads per row and steps of eight elements per thread: (16, 1) .. (1024, 4).
+// Threads per row and steps of eight elements per thread: (16, 1) .. (1024, 4).  As few threads as hold the row in one
+// step: their sums need fewer exchanges and no lanes idle (gradients of 30011 x 1000 in bfloat16 57 us with 128
+// threads, 91 us with 256).
 template <int MOST, typename Fn>
 int by_width_of_row(int width, Fn&& fn) {
     using std::integral_constant;

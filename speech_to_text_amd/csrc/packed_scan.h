@@ -817,8 +817,7 @@ struct ScanStep {
 // Entries that name the same slot are successive tokens of that sequence and are taken by the first of
 // them; a slot outside the pool gives a zero row and touches no state.  A thread has four states of a channel for
 // NE entries: their loads, which need the slots alone, go out together and before the list of slots is looked
-// through (a wavefront with one entry waits more than it moves: 3.2 TB/s), and A is read once for them
-// (256 x 4096 x 16: 32 us, 4.3 TB/s).
+// through.  256 x 4096 x 16: 28 us, 5.0 TB/s; the look through a list of 16384 takes longer than the states.
 template <typename T, int NP, int NE>
 __global__ __launch_bounds__(256) void k_scan_step(const ScanStep a) {
     using M = typename T::mem;
@@ -856,18 +855,7 @@ __global__ __launch_bounds__(256) void k_scan_step(const ScanStep a) {
     for (int k = 0; k < NE; ++k) token(k, min(e0 + k, a.batch - 1));
     load_vec<float, 4>(A2, a.A + (int64_t)c * a.state + n0, left);
     const float bias = a.bias ? a.bias[c] : 0.0f, skip = a.D ? a.D[c] : 0.0f;
-    if (a.slots) {
-        for (int i = threadIdx.x & 63; i < a.batch; i += WAVE) {
-            const int other = a.slots[i];
-#pragma unroll
-            for (int k = 0; k < NE; ++k) {
-                skipped[k] |= other == slot[k] && i < e0 + k;
-                again[k] |= other == slot[k] && i > e0 + k;
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < NE; ++k) { skipped[k] = __ballot(skipped[k]) != 0; again[k] = __ballot(again[k]) != 0; }
-    }
+    if (a.slots) slot_use<NE>(skipped, again, a.slots, a.batch, e0, slot);
 #pragma unroll
     for (int n = 0; n < 4; ++n) A2[n] *= SCAN_LOG2E;
     M* y = static_cast<M*>(a.y) + c;
@@ -923,23 +911,26 @@ inline int sum_slices(int state, bool back) { return (int)ceil_div(state, sum_st
 // Rows per chunk of the forward pass.  A chunk costs 16 bytes per state of traffic between the passes, so
 // long ones are preferred while they leave about four wavefronts for every SIMD (256 CUs x 4).  Smaller problems
 // are bound by the time of one wavefront, which goes with its rows (0.6 us each), and take shorter chunks; up to
-// 32 rows one pass is faster than three launches.
+// 32 rows one pass is faster than three launches.  With 16 rows throughout, 128 throughout, and so: 1187 x 518 x 16
+// 31, 107 and 31 us, 12007 x 2048 x 16 350, 238 and 234 us.
 inline int scan_fwd_chunk(const mfcc_scan_args* a) {
     if (a->rows <= 32) return 32;
     const int64_t waves = (int64_t)a->groups * ceil_div(a->channels / a->groups, WAVE);
     for (int chunk : {256, 128, 64})
         if (waves * ceil_div(a->rows, chunk) >= 4 * 1024) return chunk;
     if (waves * ceil_div(a->rows, 32) >= 768) return 32;
-    return waves * ceil_div(a->rows, 16) >= 1024 ? 16 : 8;
+    return waves * ceil_div(a->rows, 16) >= 512 ? 16 : 8;
 }
 
+// Rows per chunk of the gradients, by the same trade.  16 rows throughout, as many as fit, and so: 1187 x 518 x 16
+// 43, 73 and 44 us; 12007 x 2048 x 16 761, 595 and 595 us; 300 x 256 x 16, where so is 8: 31, 64 and 29 us.
 inline int bwd_channels_of(int np) { return 4 * WAVE / (np / 4); }
 inline int scan_bwd_chunk(const mfcc_scan_args* a) {
     const int cpb = bwd_channels_of(padded_state(a->state)), most = cpb >= 256 ? 16 : cpb >= 128 ? 32 : 64;
     const int64_t blocks = (int64_t)a->groups * ceil_div(a->channels / a->groups, cpb);
     int chunk = most;
-    while (chunk > 8 && blocks * ceil_div(a->rows, chunk) < 1024) chunk /= 2;
-    return chunk;
+    while (chunk > 16 && blocks * ceil_div(a->rows, chunk) < 1024) chunk /= 2;
+    return blocks * ceil_div(a->rows, 16) < 512 ? 8 : chunk;
 }
 
 inline size_t round256(size_t v) { return (v + 255) / 256 * 256; }
@@ -1004,6 +995,7 @@ int scan_empties(const mfcc_scan_args* a, const float* from, float* to, hipStrea
 template <typename T>
 void launch_carry(const Scan& f, unsigned directions, hipStream_t st) {
     const dim3 grid((unsigned)ceil_div((int64_t)f.state * f.channels, 64), directions);
+    // 1187 x 518 x 16 (75 chunks) 7 and 11 us; 2500 x 700 (157) 16 and 13, 12007 x 2048 (188) 32 and 28 us
     if (f.n_chunks <= 16 * 8) hipLaunchKernelGGL((k_scan_carry<T, 8>), grid, dim3(1024), 0, st, f);
     else hipLaunchKernelGGL((k_scan_carry<T, 16>), grid, dim3(1024), 0, st, f);
 }
@@ -1052,7 +1044,8 @@ int scan_backward(const mfcc_scan_args* a, hipStream_t st) {
             f.blocks_per_group = (int)ceil_div(f.per, bwd_channels<NP>());
             const int64_t grid2 = (int64_t)f.groups * f.blocks_per_group * f.n_chunks;
             if (grid2 > 0x7fffff) return mfcc_detail::fail(MFCC_E_UNSUPPORTED, "batch too large: split it");
-            // chunks of up to sixteen rows in a kernel with LDS for as many: three times the workgroups per CU
+            // chunks of up to sixteen rows in a kernel with LDS for as many: three times the workgroups per CU (the
+            // gradients of 1187 x 518 x 13 in float32 61 -> 53 us)
             if (f.chunk <= 16) hipLaunchKernelGGL((k_scan_bwd<T, NP, 16>), dim3((unsigned)grid2), dim3(256), 0, st, f);
             else hipLaunchKernelGGL((k_scan_bwd<T, NP, bwd_rows<NP>()>), dim3((unsigned)grid2), dim3(256), 0, st, f);
             PACKED_LAUNCHED();
@@ -1088,8 +1081,9 @@ int scan_step(const mfcc_scan_args* a, int n_slots, const int32_t* slots, hipStr
     return by_state(a->state, [&](auto np) {
         constexpr int NP = decltype(np)::value;
         const int64_t tiles = ceil_div((int64_t)a->channels * (NP / 4), 256);
-        // four entries per thread once that still leaves sixteen wavefronts for every SIMD
-        if (tiles * f.batch >= 4 * 16 * 256)
+        // four entries per thread share A and one look through the list of slots: 2048 x 1024 60 -> 51 us, but
+        // 256 x 4096 28 -> 29 us and 8 x 512 3.2 -> 4.8 us
+        if (f.batch >= 512)
             hipLaunchKernelGGL((k_scan_step<T, NP, 4>), dim3((unsigned)tiles, (unsigned)ceil_div(f.batch, 4)), dim3(256), 0, st, f);
         else
             hipLaunchKernelGGL((k_scan_step<T, NP, 1>), dim3((unsigned)tiles, (unsigned)f.batch), dim3(256), 0, st, f);

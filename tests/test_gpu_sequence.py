@@ -382,6 +382,38 @@ def test_infinite_rows_stay_in_their_sequence(gpu):
         assert torch.equal(a[39:], b[39:])
 
 
+@pytest.mark.parametrize("batch,pool", [(65, 40), (300, 500), (700, 90), (2050, 2000)])
+def test_long_lists_of_slots(gpu, batch, pool):
+    """Entries that name one slot, anywhere in a list of any length, give what one call per occurrence gives."""
+    import speech_to_text_amd as S
+
+    g = gen(gpu, batch)
+    ch, n, width = 70, 9, 3
+    slots = torch.randint(-3, pool + 3, (batch,), generator=torch.Generator().manual_seed(batch))
+    seen, turn = {}, []
+    for s in slots.tolist():
+        seen[s] = seen.get(s, -1) + 1
+        turn.append(seen[s])
+    turn = torch.tensor(turn)
+    u, delta = randn(g, batch, ch, dtype=BF16), randn(g, batch, ch, dtype=BF16)
+    b, c = randn(g, batch, n, dtype=BF16), randn(g, batch, n, dtype=BF16)
+    A, w = -rand(g, ch, n, lo=0.1, hi=2.0), randn(g, ch, width)
+    h0, x0 = randn(g, pool, ch, n), randn(g, pool, width - 1, ch, dtype=BF16)
+    h, line = h0.clone(), x0.clone()
+    dev = slots.to(gpu, torch.int32)
+    y = S.selective_scan_step(u, delta, A, b, c, h, softplus=True, slots=dev)
+    z = S.causal_conv_step(u, line, w, slots=dev)
+    h1, line1, y1, z1 = h0.clone(), x0.clone(), torch.empty_like(y), torch.empty_like(z)
+    for k in range(int(turn.max()) + 1):
+        i = (turn == k).nonzero().flatten().to(gpu)
+        part = [t[i] for t in (u, delta, b, c)]
+        y1[i] = S.selective_scan_step(part[0], part[1], A, part[2], part[3], h1, softplus=True, slots=dev[i])
+        z1[i] = S.causal_conv_step(part[0], line1, w, slots=dev[i])
+    assert torch.equal(y, y1) and torch.equal(h, h1) and torch.equal(z, z1) and torch.equal(line, line1)
+    outside = (slots < 0) | (slots >= pool)
+    assert outside.any() and (y[outside.to(gpu)] == 0).all() and (z[outside.to(gpu)] == 0).all()
+
+
 # ---- norms ---------------------------------------------------------------------------------------------------------
 NORMS = [(1, 1), (3, 7), (9, 64), (5, 513), (2, 1000), (70, 96), (4, 2049), (3, 4100), (2, 9001), (1, 20000), (300, 40),
          (6, 1500), (77, 200), (3, 7000),
