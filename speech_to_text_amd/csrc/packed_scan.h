@@ -426,15 +426,16 @@ __global__ __launch_bounds__(256) void k_scan_fwd(const Scan a) {
 }
 
 // Sequences without rows (and those whose offsets do not lie within the rows): the state passes through,
-// and so does its gradient.
-template <typename T>
-__global__ __launch_bounds__(256) void k_scan_empty(const int64_t* __restrict__ off, int64_t rows, int64_t size,
-                                                    const float* __restrict__ from, float* __restrict__ to) {
-    const int64_t s = blockIdx.x;
-    const int64_t start = off ? off[s] : 0, end = off ? min(off[s + 1], rows) : rows;
+// and so does its gradient.  A workgroup takes the elements first, first + step, ... of sequence s.
+struct Empties { const int64_t* off; int64_t rows, size; const float* from; float* to; };
+__device__ __forceinline__ void pass_through(const Empties& a, int64_t s, int64_t first, int64_t step) {
+    const int64_t start = a.off ? a.off[s] : 0, end = a.off ? min(a.off[s + 1], a.rows) : a.rows;
     if (start >= 0 && start < end) return;
-    for (int64_t i = (int64_t)blockIdx.y * 256 + threadIdx.x; i < size; i += (int64_t)gridDim.y * 256)
-        to[s * size + i] = from ? from[s * size + i] : 0.0f;
+    for (int64_t i = first; i < a.size; i += step) a.to[s * a.size + i] = a.from ? a.from[s * a.size + i] : 0.0f;
+}
+template <typename T>
+__global__ __launch_bounds__(1024) void k_scan_empty(const Empties a) {
+    pass_through(a, blockIdx.x, threadIdx.x, 1024);
 }
 
 // ---- gradients ---------------------------------------------------------------------------------------
@@ -765,7 +766,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(bwd_waves<T
     if (a.part_bias) fold(db, a.part_bias);
 }
 
-// The sums of the partial results, one launch for all of them: out[e] = sum over parts of part[p][e], of rows of
+// The sums of the partial results, one launch for all of them and, in the blocks behind sum_blocks, for the initial
+// states of sequences without rows: out[e] = sum over parts of part[p][e], of rows of
 // `padded` columns of which the first `inner` are kept.  64 elements by 16 slices of the parts.  17 us for the
 // 65 MB of 12007 x 2048 x 16.
 struct ReduceJob {
@@ -773,12 +775,16 @@ struct ReduceJob {
     int64_t n_part, m, first_block;
     int padded, inner, wide;             // wide: out is float32, else of the element type
 };
-struct ReduceJobs { ReduceJob job[5]; int count; };
+struct ReduceJobs { ReduceJob job[5]; int count; int64_t sum_blocks; Empties empties; };
 
 template <typename T>
 __global__ __launch_bounds__(1024) void k_scan_reduce(const ReduceJobs jobs) {
     using M = typename T::mem;
     __shared__ float sh[16][64];
+    if (blockIdx.x >= jobs.sum_blocks) {
+        pass_through(jobs.empties, blockIdx.x - jobs.sum_blocks, threadIdx.x, 1024);
+        return;
+    }
     int which = 0;
     for (int i = 1; i < jobs.count; ++i)
         if (blockIdx.x >= jobs.job[i].first_block) which = i;
@@ -982,14 +988,11 @@ inline Scan scan_args(const mfcc_scan_args* a, bool back) {
     return f;
 }
 
-template <typename T>
-int scan_empties(const mfcc_scan_args* a, const float* from, float* to, hipStream_t st) {
-    if (!to || a->n_seqs == 0 || (!a->d_offsets && a->rows > 0)) return MFCC_OK;
-    const int64_t size = (int64_t)a->channels * a->state;
-    hipLaunchKernelGGL(k_scan_empty<T>, dim3((unsigned)a->n_seqs, (unsigned)std::min<int64_t>(ceil_div(size, 256), 64)), dim3(256),
-                       0, st, a->d_offsets, a->rows, size, from, to);
-    PACKED_LAUNCHED();
-    return MFCC_OK;
+// The sequences that pass_through has to look at: all of them, or none.
+inline int scan_empties(const mfcc_scan_args* a, const float* from, float* to, Empties* e) {
+    if (!to || (!a->d_offsets && a->rows > 0)) return 0;
+    *e = {a->d_offsets, a->rows, (int64_t)a->channels * a->state, from, to};
+    return a->n_seqs;
 }
 
 template <typename T>
@@ -1006,7 +1009,7 @@ int scan_forward(const mfcc_scan_args* a, hipStream_t st) {
     const int block = scan_block(f.per);
     f.blocks_per_group = (int)ceil_div(f.per, block);
     const int64_t grid = (int64_t)f.groups * f.blocks_per_group * f.n_chunks;
-    if (grid > 0x7fffff) return mfcc_detail::fail(MFCC_E_UNSUPPORTED, "batch too large: split it");
+    if (grid > 0x7fffff || (a->d_final && a->n_seqs > 0x3fffff)) return mfcc_detail::fail(MFCC_E_UNSUPPORTED, "batch too large: split it");
     if (a->rows > 0) {
         const int rc = by_state(a->state, [&](auto np) {
             constexpr int NP = decltype(np)::value;
@@ -1022,7 +1025,12 @@ int scan_forward(const mfcc_scan_args* a, hipStream_t st) {
         });
         if (rc) return rc;
     }
-    return scan_empties<T>(a, a->d_initial, a->d_final, st);
+    Empties e;
+    if (const int seqs = scan_empties(a, a->d_initial, a->d_final, &e)) {
+        hipLaunchKernelGGL(k_scan_empty<T>, dim3((unsigned)seqs), dim3(1024), 0, st, e);
+        PACKED_LAUNCHED();
+    }
+    return MFCC_OK;
 }
 
 template <typename T>
@@ -1063,10 +1071,12 @@ int scan_backward(const mfcc_scan_args* a, hipStream_t st) {
         reduce(f.part_A, f.n_chunks, (int64_t)f.channels * NP, NP, f.state, a->d_dA, true);
         reduce(f.part_D, f.n_chunks, f.channels, 1, 1, a->d_dD, true);
         reduce(f.part_bias, f.n_chunks, f.channels, 1, 1, a->d_ddelta_bias, true);
-        if (blocks > 0x3fffff) return mfcc_detail::fail(MFCC_E_UNSUPPORTED, "batch too large: split it");
+        jobs.sum_blocks = blocks;
+        blocks += scan_empties(a, a->d_dfinal, a->d_dinitial, &jobs.empties);
+        if (blocks > 0x1fffff) return mfcc_detail::fail(MFCC_E_UNSUPPORTED, "batch too large: split it");
         hipLaunchKernelGGL(k_scan_reduce<T>, dim3((unsigned)blocks), dim3(1024), 0, st, jobs);
         PACKED_LAUNCHED();
-        return scan_empties<T>(a, a->d_dfinal, a->d_dinitial, st);
+        return (int)MFCC_OK;
     });
 }
 
