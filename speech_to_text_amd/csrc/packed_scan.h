@@ -12,7 +12,8 @@
 // Bound by vector issue, not memory: per (row, channel, n) one exp (8 SIMD cycles per wavefront) and four to
 // five plain operations (2.6 each) per pass against 6 / N bytes in 16-bit types.  16384 x 2048, 16 states, bfloat16:
 // 116 + 10 + 147 us for the three passes (the two sweeps 4.6 and 3.7 10^12 elements (row, channel, n) a second).
-// The first sweep is what the split costs; undivided, 2048 channels are 32 wavefronts for 1024 SIMDs.
+// In both 80 % of the issue slots are taken.  The first sweep is what the split costs; undivided, 2048 channels are
+// 32 wavefronts for 1024 SIMDs.
 #pragma once
 #include "packed.h"
 
@@ -450,8 +451,8 @@ __global__ __launch_bounds__(1024) void k_scan_empty(const Empties a) {
 // latencies overlap.  Sums over n stay in the LPC lanes of a channel; dB and dC are summed over the channels of the
 // wavefront (v_permlane swaps halve eight values to two, then rotations within a row of lanes), over the four
 // wavefronts in LDS, and over the workgroups of a group by k_scan_reduce: a fixed order throughout.
-// Bound by vector issue: 113 instructions per wavefront and row (256 elements), two of eight an exp; the vector units
-// are busy 91 % of the time.  12007 x 2048 x 16 in bfloat16: 415 us.
+// Bound by vector issue: 113 instructions per wavefront and row (256 elements), eight of them an exp; 80 % of
+// the issue slots are taken (an exp takes two).  12007 x 2048 x 16 in bfloat16: 415 us.
 constexpr int SUB = 8;
 
 template <int NP> constexpr int bwd_lpc() { return NP / 4; }
@@ -1052,8 +1053,8 @@ int scan_backward(const mfcc_scan_args* a, hipStream_t st) {
             f.blocks_per_group = (int)ceil_div(f.per, bwd_channels<NP>());
             const int64_t grid2 = (int64_t)f.groups * f.blocks_per_group * f.n_chunks;
             if (grid2 > 0x7fffff) return mfcc_detail::fail(MFCC_E_UNSUPPORTED, "batch too large: split it");
-            // chunks of up to sixteen rows in a kernel with LDS for as many: three times the workgroups per CU (the
-            // gradients of 1187 x 518 x 13 in float32 61 -> 53 us)
+            // chunks of up to sixteen rows in a kernel with LDS and registers for as many: more workgroups per CU
+            // (the gradients of 1187 x 518 x 13 in float32 61 -> 53 us)
             if (f.chunk <= 16) hipLaunchKernelGGL((k_scan_bwd<T, NP, 16>), dim3((unsigned)grid2), dim3(256), 0, st, f);
             else hipLaunchKernelGGL((k_scan_bwd<T, NP, bwd_rows<NP>()>), dim3((unsigned)grid2), dim3(256), 0, st, f);
             PACKED_LAUNCHED();
