@@ -538,7 +538,7 @@ def test_gradients_of_more_wide_rows_than_workgroups(gpu):
         want += n.sum(0)
         size += n.abs().sum(0)
     # each value's own error (the gate's and the norm's, as in the smaller cases), and the sum: a chain of rows / workgroups
-    # (409, of five tiles in 2048) in each partial sum and of 16 slices over them
+    # (409, of five tiles in 2048) in each partial sum and of at least 16 slices over them
     R.assert_close(got.weight, want.cpu(), F32, size.cpu(), rows / 409 + 409 / 16 + 20 + 2 * (ch / 64 + 34), "weight")
 
 
