@@ -296,8 +296,7 @@ __global__ __launch_bounds__(256) void k_conv_bwd(const ConvBwd a) {
                 }
             }
 #pragma unroll
-            for (int j = 0; j < K - 1; ++j)
-{
+            for (int j = 0; j < K - 1; ++j) {
                 line[j] = line[j + GROUP];
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) dp[j][i] = dp[j + GROUP][i];
@@ -473,12 +472,15 @@ inline int conv_fwd_tile(int64_t rows, int n_vec) {
     return 8;
 }
 
-// Rows per wavefront of the backward pass (it also writes K + 1 partial sums per four tiles).  16 rows throughout, 128
-// throughout, and so, with the summing launch: 600 x 512 20, 86 and 20 us; 30011 x 4096 185, 183 and 182 us.
+// Rows per wavefront of the backward pass (it also reads K - 1 rows of overlap and writes K + 1 partial sums per four
+// tiles).  K = 4, bfloat16, with the summing launch, by tiles of 4, 8, 16 and 128 rows: 600 x 512 11.7, 15, 20, 86 us;
+// 4000 x 1024 20.1, 19.4, 22, 88; 12000 x 1024 38, 32, 29, -; 30011 x 4096 -, -, 185, 183.
 inline int conv_bwd_tile(int64_t rows, int n_vec) {
+    const int64_t across = ceil_div(n_vec, WAVE);
     for (int tile : {128, 64, 32})
-        if (ceil_div(rows, tile) * ceil_div(n_vec, WAVE) >= 4 * 1024) return tile;
-    return 16;
+        if (ceil_div(rows, tile) * across >= 4 * 1024) return tile;
+    const int64_t waves = ceil_div(rows, 16) * across;
+    return waves >= 2048 ? 16 : waves >= 512 ? 8 : 4;
 }
 
 inline int64_t conv_bwd_parts(const mfcc_conv_args* a) {

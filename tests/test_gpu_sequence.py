@@ -599,8 +599,9 @@ def scan64(u, d, A, B, C, dy, off, rate):
 
 
 @pytest.mark.parametrize("rows,ch,n", [
-    (16500, 4096, 1), (8300, 4096, 2), (4200, 4096, 3), (1500, 704, 4), (900, 700, 5),     # forward 256, 128, 64, 16 and 8 rows
-    (1100, 4096, 16), (2100, 1024, 16), (1600, 1024, 16), (1200, 640, 16)])                # gradient 64, 32, 16 and 8; forward 32
+    (16500, 4096, 1), (8300, 4096, 2), (4200, 4096, 3), (1500, 704, 4), (900, 700, 5),     # forward 256, 128, 64 and 16 rows
+    (1100, 4096, 16), (2100, 1024, 16), (1600, 1024, 16), (1200, 640, 16),                 # gradient 64, 32 and 16; forward 32
+    (600, 512, 16)])                                                                       # both 8
 def test_scan_of_every_chunk_length(gpu, rows, ch, n):
     import speech_to_text_amd as S
 
@@ -626,9 +627,9 @@ def test_scan_of_every_chunk_length(gpu, rows, ch, n):
         R.assert_close(got, want[name].cpu(), kind, size[name].cpu(), steps + extra, name)
 
 
-@pytest.mark.parametrize("rows", [9000, 17000, 34000, 66000])
+@pytest.mark.parametrize("rows", [9000, 17000, 34000, 66000, 2010, 3000])
 def test_causal_conv_of_every_tile(gpu, rows):
-    """Sizes at which a thread of the forward pass takes 16, 32, 64 and 128 rows, of the gradient 32, 64 and 128."""
+    """Sizes at which a thread of the forward pass takes 16, 32, 64, 128 and 8 rows, of the gradient 32, 64, 128, 8 and 16."""
     import speech_to_text_amd as S
 
     g = gen(gpu, rows)
