@@ -20,7 +20,7 @@ struct ConvFwd {
     const void* initial;
     void* y; int64_t y_stride;
     int64_t rows; int n_seqs, channels, n_vec, tile;
-    int zero_rest, act;
+    int zero_rest, act, room;
 };
 
 // The taps and biases of the thread's channels (neighbours in memory).
@@ -74,12 +74,14 @@ __global__ __launch_bounds__(256) void k_conv_fwd(const ConvFwd a) {
 
     Raw<M, VEC> line[K - 1 + G], next[G];
     auto fetch = [&](int64_t r) {
+        const bool room = a.room && (r1 < a.rows || r + G < a.rows);
 #pragma unroll
-        for (int g = 0; g < G; ++g) load_raw<M, VEC>(next[g], x + min(r + g, r1 - 1) * a.x_stride, n);
+        for (int g = 0; g < G; ++g) load_raw<M, VEC>(next[g], x + min(r + g, r1 - 1) * a.x_stride, n, room);
     };
     fetch(r0);
 #pragma unroll
-    for (int j = 0; j < K - 1; ++j) load_raw<M, VEC>(line[j], x + max(r0 - (K - 1) + j, (int64_t)0) * a.x_stride, n);
+    for (int j = 0; j < K - 1; ++j)
+        load_raw<M, VEC>(line[j], x + max(r0 - (K - 1) + j, (int64_t)0) * a.x_stride, n, a.room && a.rows > 1);
     float w[K][VEC], b[VEC];
     load_taps<K, VEC>(w, b, a.w, a.bias, c0, n);
     Place q = find_row(a.off, a.n_seqs, a.rows, r0);
@@ -173,7 +175,7 @@ struct ConvBwd {
     void* dx; int64_t dx_stride;
     float* part;                 // (row tiles / 4, K + 1, channels): sums for dweight and dbias
     void* dinitial;
-    int64_t rows; int n_seqs, channels, n_vec, tile, act;
+    int64_t rows; int n_seqs, channels, n_vec, tile, act, room;
 };
 
 // dp = dy * act'(p) is formed for the tile's rows and the K - 1 rows behind it; dx[o] gathers the K values
@@ -203,17 +205,18 @@ __global__ __launch_bounds__(256) void k_conv_bwd(const ConvBwd a) {
         Raw<M, VEC> line[K - 1 + GROUP], dyr[GROUP], next_x[GROUP], next_dy[GROUP];
         float dp[K - 1 + GROUP][VEC];
         auto fetch = [&](int64_t r) {
+            const bool room = a.room && r + GROUP < a.rows;
 #pragma unroll
             for (int g = 0; g < GROUP; ++g) {
                 const int64_t row = min(r + g, a.rows - 1);
-                load_raw<M, VEC>(next_x[g], x + row * a.x_stride, n);
-                load_raw<M, VEC>(next_dy[g], dy + row * a.dy_stride, n);
+                load_raw<M, VEC>(next_x[g], x + row * a.x_stride, n, room);
+                load_raw<M, VEC>(next_dy[g], dy + row * a.dy_stride, n, room);
             }
         };
         fetch(r0);
 #pragma unroll
         for (int j = 0; j < K - 1; ++j) {
-            load_raw<M, VEC>(line[j], x + max(r0 - (K - 1) + j, (int64_t)0) * a.x_stride, n);
+            load_raw<M, VEC>(line[j], x + max(r0 - (K - 1) + j, (int64_t)0) * a.x_stride, n, a.room && a.rows > 1);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) dp[j][i] = 0.0f;    // rows before the tile: their dx belongs to the tile above
         }
@@ -515,6 +518,7 @@ int conv_forward(const mfcc_conv_args* a, hipStream_t st) {
             f.initial = a->d_initial; f.y = a->d_y; f.y_stride = a->y_stride; f.rows = a->rows;
             f.n_seqs = a->n_seqs; f.channels = a->channels; f.n_vec = (int)ceil_div(a->channels, VEC);
             f.tile = conv_fwd_tile(a->rows, f.n_vec); f.zero_rest = a->zero_rest; f.act = a->activation == MFCC_ACT_SILU;
+            f.room = has_room(f.x, f.x_stride, VEC);
             const int64_t blocks = ceil_div(ceil_div(a->rows, f.tile) * f.n_vec, 256);
             if (blocks > 0x7fffff) return mfcc_detail::fail(MFCC_E_UNSUPPORTED, "batch too large: split it");
             hipLaunchKernelGGL((k_conv_fwd<T, K, VEC, CONV_AHEAD>), dim3((unsigned)blocks), dim3(256), 0, st, f);
@@ -542,6 +546,7 @@ int conv_backward(const mfcc_conv_args* a, hipStream_t st) {
         f.dx_stride = a->dx_stride; f.part = static_cast<float*>(a->d_workspace); f.dinitial = a->d_dinitial;
         f.rows = a->rows; f.n_seqs = a->n_seqs; f.channels = a->channels; f.act = a->activation == MFCC_ACT_SILU;
         f.n_vec = (int)ceil_div(a->channels, CONV_VEC); f.tile = conv_bwd_tile(a->rows, f.n_vec);
+        f.room = has_room(f.x, f.x_stride, CONV_VEC) && has_room(f.dy, f.dy_stride, CONV_VEC);
         const int64_t parts = conv_bwd_parts(a);
         if (parts > 65535) return mfcc_detail::fail(MFCC_E_UNSUPPORTED, "batch too large: split it");
         if (a->rows > 0) {

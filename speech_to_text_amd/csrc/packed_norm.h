@@ -24,7 +24,7 @@ struct Norm {
     float* part;               // (blocks, 3, channels): dweight, dbias, dscale
     float4* stats;             // wide rows: mean, 1 / deviation, and their gradient's (rows, groups)
     int64_t rows;
-    int channels, groups, width, layer, gate_first;
+    int channels, groups, width, layer, gate_first, room;
     bool want[3];              // of the three sums
     float eps, scale_value, inv_width;
 };
@@ -46,8 +46,8 @@ __device__ __forceinline__ void unit_sum2(float& a, float& b, float (*sh)[2]) {
 }
 
 template <typename M>
-__device__ __forceinline__ void load_or(float (&v)[NV], const M* p, int n, float other) {
-    if (p) load_vec<M, NV>(v, p, n);
+__device__ __forceinline__ void load_or(float (&v)[NV], const M* p, int n, float other, bool room = false) {
+    if (p) load_vec<M, NV>(v, p, n, room);
     else {
 #pragma unroll
         for (int i = 0; i < NV; ++i) v[i] = other;
@@ -71,10 +71,11 @@ __global__ __launch_bounds__(norm_block(TPU)) void k_norm_fwd(const Norm a) {
 #pragma unroll
     for (int k = 0; k < IT; ++k) {
         const int w0 = (k * TPU + tid) * NV, c = c_base + w0, n = max(a.width - w0, 0);
+        const bool room = a.room && row + 1 < a.rows;
         float xv[NV];
-        load_vec<M, NV>(xv, x + c, n);
+        load_vec<M, NV>(xv, x + c, n, room);
         if (GATE) {
-            load_vec<M, NV>(gate[k], static_cast<const M*>(a.z) + row * a.z_stride + c, n);
+            load_vec<M, NV>(gate[k], static_cast<const M*>(a.z) + row * a.z_stride + c, n, room);
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 gate[k][i] *= sigmoid_f(gate[k][i]);
@@ -83,13 +84,15 @@ __global__ __launch_bounds__(norm_block(TPU)) void k_norm_fwd(const Norm a) {
         } else {
             float sc[NV], rv[NV];
             load_or<float>(sc, a.scale ? a.scale + c : nullptr, n, a.scale_value);
-            load_or<RM>(rv, a.residual ? static_cast<const RM*>(a.residual) + row * a.residual_stride + c : nullptr, n, 0.0f);
+            load_or<RM>(rv, a.residual ? static_cast<const RM*>(a.residual) + row * a.residual_stride + c : nullptr, n, 0.0f, room);
 #pragma unroll
             for (int i = 0; i < NV; ++i) v[k][i] = fmaf(sc[i], xv[i], rv[i]);
-            if (n < NV) {
+        }
+        if (n < NV) {
 #pragma unroll
-                for (int i = 0; i < NV; ++i) v[k][i] = i < n ? v[k][i] : 0.0f;
-            }
+            for (int i = 0; i < NV; ++i) v[k][i] = i < n ? v[k][i] : 0.0f;
+        }
+        if (!GATE) {
             if (a.r && n > 0) store_vec<RM, NV>(static_cast<RM*>(a.r) + row * a.r_stride + c, v[k], n);
         }
 #pragma unroll
@@ -131,8 +134,11 @@ __global__ __launch_bounds__(norm_block(TPU)) void k_norm_fwd(const Norm a) {
 // one partial row per block is written and k_norm_reduce adds those in a fixed order.  With eight elements a thread
 // (IT = 1) the tables stay in registers and the next row is in flight during the reductions of the current one (for
 // the gate in 16-bit types only: three float32 rows ahead cost a wavefront per SIMD, 28 against 26 us at 4099 x 1537).
+// Four wavefronts per SIMD in 16-bit types, a few registers spilled: the gate at 16384 x 2048 83 -> 72 us.
+template <typename T, int IT> constexpr int norm_bwd_waves() { return IT == 1 && sizeof(typename T::mem) == 2 ? 4 : 1; }
 template <typename T, typename RT, bool GATE, int TPU, int IT>
-__global__ __launch_bounds__(norm_block(TPU)) void k_norm_bwd(const Norm a) {
+__global__ __launch_bounds__(norm_block(TPU)) __attribute__((amdgpu_waves_per_eu(norm_bwd_waves<T, IT>())))
+void k_norm_bwd(const Norm a) {
     using M = typename T::mem;
     using RM = typename RT::mem;
     constexpr int PER = norm_block(TPU) / TPU;
@@ -149,19 +155,24 @@ __global__ __launch_bounds__(norm_block(TPU)) void k_norm_bwd(const Norm a) {
     struct RowIn { Raw<M, NV> dy[IT], x[IT], z[GATE ? IT : 1]; Raw<RM, NV> r[GATE ? 1 : IT], dr[GATE ? 1 : IT]; };
     auto fetch = [&](RowIn& in, int64_t row) {
         const float zero[NV] = {};
+        const bool room = a.room && row + 1 < a.rows;
 #pragma unroll
         for (int k = 0; k < IT; ++k) {
-            const int c = col(k), n = left(k);
-            if (a.dy) load_raw<M, NV>(in.dy[k], static_cast<const M*>(a.dy) + row * a.dy_stride + c, n);
-            else in.dy[k].set(zero);
-            if (GATE || a.x) load_raw<M, NV>(in.x[k], static_cast<const M*>(a.x) + row * a.x_stride + c, n);
-            if (GATE) {
-                load_raw<M, NV>(in.z[GATE ? k : 0], static_cast<const M*>(a.z) + row * a.z_stride + c, n);
-            } else {
-                load_raw<RM, NV>(in.r[GATE ? 0 : k], static_cast<const RM*>(a.r_in) + row * a.r_stride + c, n);
-                if (a.dr) load_raw<RM, NV>(in.dr[GATE ? 0 : k], static_cast<const RM*>(a.dr) + row * a.dr_stride + c, n);
-                else in.dr[GATE ? 0 : k].set(zero);
-            }
+            const int c = col(k), all = left(k);
+            auto take = [&](int n) {
+                if (a.dy) load_raw<M, NV>(in.dy[k], static_cast<const M*>(a.dy) + row * a.dy_stride + c, n);
+                else in.dy[k].set(zero);
+                if (GATE || a.x) load_raw<M, NV>(in.x[k], static_cast<const M*>(a.x) + row * a.x_stride + c, n);
+                if (GATE) {
+                    load_raw<M, NV>(in.z[GATE ? k : 0], static_cast<const M*>(a.z) + row * a.z_stride + c, n);
+                } else {
+                    load_raw<RM, NV>(in.r[GATE ? 0 : k], static_cast<const RM*>(a.r_in) + row * a.r_stride + c, n);
+                    if (a.dr) load_raw<RM, NV>(in.dr[GATE ? 0 : k], static_cast<const RM*>(a.dr) + row * a.dr_stride + c, n);
+                    else in.dr[GATE ? 0 : k].set(zero);
+                }
+            };
+            if (all >= NV || (room && all > 0)) take(NV);
+            else take(all);
         }
     };
     // weight, and the bias (gate) or the scale (add)
@@ -514,6 +525,8 @@ inline Norm norm_args(const mfcc_norm_args* a) {
     f.dz = a->d_dz; f.dresidual = a->d_dresidual; f.rows = a->rows; f.channels = a->channels; f.groups = a->groups;
     f.width = a->channels / a->groups; f.layer = a->norm == MFCC_NORM_LAYER; f.gate_first = a->gate_first;
     f.eps = a->eps; f.scale_value = a->scale_value; f.inv_width = 1.0f / (float)f.width;
+    f.room = has_room(f.x, f.x_stride, NV) && has_room(f.z, f.z_stride, NV) && has_room(f.residual, f.residual_stride, NV) &&
+             has_room(f.r_in, f.r_stride, NV) && has_room(f.dy, f.dy_stride, NV) && has_room(f.dr, f.dr_stride, NV);
     return f;
 }
 

@@ -573,6 +573,43 @@ def test_norms_of_special_rows(gpu):
     assert (S.add_norm_backward(none, None, none, w).weight == 0).all()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,ch,how", [(70, 45, "nan"), (70, 1001, "nan"), (33, 2, "nan"), (9, 2050, "nan"), (1, 45, "nan"),
+                                         (70, 45, "expanded"), (5, 3, "expanded"), (41, 1, "expanded")])
+def test_what_lies_behind_a_row(gpu, rows, ch, how, dtype):
+    """Column ranges of a wider matrix with NaN around them, and one row expanded to many, as their contiguous copies."""
+    import speech_to_text_amd as S
+
+    g = gen(gpu, rows + ch)
+
+    def tensor():
+        if how == "expanded":
+            return randn(g, 1, ch, dtype=dtype).expand(rows, ch)
+        around = torch.full((rows, ch + 9), float("nan"), dtype=dtype, device=gpu)
+        around[:, 3:3 + ch] = randn(g, rows, ch, dtype=dtype)
+        return around[:, 3:3 + ch]
+
+    def same(got, want):
+        got, want = (t if isinstance(t, tuple) else (t,) for t in (got, want))
+        for a, b in zip(got, want):
+            assert (a is None and b is None) or (torch.isfinite(a).all() and torch.equal(a, b))
+
+    x, z, dy, dr = (tensor() for _ in range(4))
+    plain = [t.contiguous() for t in (x, z, dy, dr)]
+    w, b, taps, scale = randn(g, ch), randn(g, ch), randn(g, ch, 4), rand(g, ch, lo=0.2, hi=1.5)
+    call = lambda f: same(f(x, z, dy, dr), f(*plain))
+    call(lambda x, z, dy, dr: S.causal_conv(x, taps, b, activation="silu", return_state=True))
+    call(lambda x, z, dy, dr: S.causal_conv_backward(dy, x, taps, b, activation="silu"))
+    for kind in ("rms", "layer"):
+        call(lambda x, z, dy, dr: S.add_norm(x, z, w, b, scale=scale, norm=kind))
+        call(lambda x, z, dy, dr: S.add_norm_backward(dy, dr, z, w, b, x=x, scale=scale, norm=kind))
+        for first in (True, False):
+            for groups in (1, ch):
+                if groups == 1 or ch < 50:
+                    call(lambda x, z, dy, dr: S.gate_norm(x, z, w, b, norm=kind, gate_first=first, groups=groups))
+                    call(lambda x, z, dy, dr: S.gate_norm_backward(dy, x, z, w, b, norm=kind, gate_first=first, groups=groups))
+
+
 # ---- every choice of tile and chunk ------------------------------------------------------------------------------------
 def scan64(u, d, A, B, C, dy, off, rate):
     """Values and gradients row by row in 64 bits on the GPU; `rate` is A, or |A| for magnitudes (d u, B, C, dy then
