@@ -472,12 +472,14 @@ __device__ __forceinline__ float sum_states(float v) {       // over the LPC nei
     return v;
 }
 
+// Over the lanes of a row of 16 with equal lane % LPC, the same bits in all of them: by 8 first, so that after every
+// step the values repeat at the next distance and the rotation adds the same two of them in either lane.
 template <int LPC>
-__device__ __forceinline__ float sum_channels(float v) {     // over the lanes of a row of 16 with equal lane % LPC
-    if (LPC <= 1) v += dpp<0x121>(v);                         // row_ror:1, 2, 4, 8
-    if (LPC <= 2) v += dpp<0x122>(v);
+__device__ __forceinline__ float sum_channels(float v) {
+    if (LPC <= 8) v += dpp<0x128>(v);                         // row_ror:8, 4, 2, 1
     if (LPC <= 4) v += dpp<0x124>(v);
-    if (LPC <= 8) v += dpp<0x128>(v);
+    if (LPC <= 2) v += dpp<0x122>(v);
+    if (LPC <= 1) v += dpp<0x121>(v);
     return v;
 }
 
@@ -703,7 +705,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(bwd_waves<T
             const float w0 = halve32(red[0], red[4]), w1 = halve32(red[1], red[5]);
             const float w2 = halve32(red[2], red[6]), w3 = halve32(red[3], red[7]);
             const float v0 = sum_channels<LPC>(halve16(w0, w2)), v1 = sum_channels<LPC>(halve16(w1, w3));
-            // all lanes of a row with the same states hold the same sums: they write one place
+            // all lanes of a row with the same states hold the same sums, bit for bit: they write one place
             *reinterpret_cast<float2*>(pslab + (s & 1) * SLAB + j * 2 * NP) = make_float2(v0, v1);
         }
         if (nq == 0) {
