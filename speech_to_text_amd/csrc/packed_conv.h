@@ -548,15 +548,14 @@ int conv_backward(const mfcc_conv_args* a, hipStream_t st) {
         f.n_vec = (int)ceil_div(a->channels, CONV_VEC); f.tile = conv_bwd_tile(a->rows, f.n_vec);
         f.room = has_room(f.x, f.x_stride, CONV_VEC) && has_room(f.dy, f.dy_stride, CONV_VEC);
         const int64_t parts = conv_bwd_parts(a);
-        if (parts > 65535) return mfcc_detail::fail(MFCC_E_UNSUPPORTED, "batch too large: split it");
+        const int64_t sum_blocks = ceil_div((int64_t)(K + 1) * a->channels, 64);
+        const int64_t more = a->d_dinitial && K > 1 ? ceil_div((int64_t)a->n_seqs * a->channels, 1024) : 0;
+        if (parts > 65535 || sum_blocks + more > 0x1fffff) return mfcc_detail::fail(MFCC_E_UNSUPPORTED, "batch too large: split it");
         if (a->rows > 0) {
             hipLaunchKernelGGL((k_conv_bwd<T, K, CONV_VEC>), dim3((unsigned)ceil_div(f.n_vec, WAVE), (unsigned)parts),
                                dim3(256), 0, st, f);
             PACKED_LAUNCHED();
         }
-        const int64_t sum_blocks = ceil_div((int64_t)(K + 1) * a->channels, 64);
-        const int64_t more = a->d_dinitial && K > 1 ? ceil_div((int64_t)a->n_seqs * a->channels, 1024) : 0;
-        if (sum_blocks + more > 0x1fffff) return mfcc_detail::fail(MFCC_E_UNSUPPORTED, "batch too large: split it");
         hipLaunchKernelGGL((k_conv_finish<T, K>), dim3((unsigned)(sum_blocks + more)), dim3(1024), 0, st, f, parts,
                            (int)sum_blocks, a->d_dweight, a->d_dbias);
         PACKED_LAUNCHED();

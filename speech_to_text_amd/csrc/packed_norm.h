@@ -551,6 +551,7 @@ int norm_backward(const mfcc_norm_args* a, hipStream_t st) {
     const int blocks = norm_bwd_blocks(a);
     f.want[0] = a->d_dweight; f.want[1] = a->d_dbias; f.want[2] = a->d_dscale;
     const bool sums = f.want[0] || f.want[1] || f.want[2];
+    if (sums && ceil_div(f.channels, 32) > 0x3fffff) return mfcc_detail::fail(MFCC_E_UNSUPPORTED, "batch too large: split it");
     const bool wide = f.width > NORM_HELD;
     if (sums) {
         f.stats = static_cast<float4*>(a->d_workspace);

@@ -735,7 +735,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(bwd_waves<T
         for (int q = 0; q < (SUB * 2 * NP + 255) / 256; ++q) {
             const int i = q * 256 + tid, j = i / (2 * NP), w = i / NP & 1;
             if (i < SUB * 2 * NP && s * SUB + j < len)
-                part_bc[w * bc_which + (s * SUB + j) * bc_row + i % NP] =
+                part_bc[w * bc_which + (int64_t)(s * SUB + j) * bc_row + i % NP] =
                     (sum4[i] + sum4[SLAB / 4 + i]) + (sum4[SLAB / 2 + i] + sum4[3 * SLAB / 4 + i]);
         }
     }
@@ -998,9 +998,13 @@ inline int scan_empties(const mfcc_scan_args* a, const float* from, float* to, E
     return a->n_seqs;
 }
 
+// A launch numbers at most 2^32 - 1 threads; every limit is looked at before the first launch of a call.
+inline int too_large() { return mfcc_detail::fail(MFCC_E_UNSUPPORTED, "batch too large: split it"); }
+inline int64_t carry_blocks(const Scan& f) { return ceil_div((int64_t)f.state * f.channels, 64); }
+
 template <typename T>
 void launch_carry(const Scan& f, unsigned directions, hipStream_t st) {
-    const dim3 grid((unsigned)ceil_div((int64_t)f.state * f.channels, 64), directions);
+    const dim3 grid((unsigned)carry_blocks(f), directions);
     // 1187 x 518 x 16 (75 chunks) 7 and 11 us; 2500 x 700 (157) 16 and 13, 12007 x 2048 (188) 32 and 28 us
     if (f.n_chunks <= 16 * 8) hipLaunchKernelGGL((k_scan_carry<T, 8>), grid, dim3(1024), 0, st, f);
     else hipLaunchKernelGGL((k_scan_carry<T, 16>), grid, dim3(1024), 0, st, f);
@@ -1012,12 +1016,12 @@ int scan_forward(const mfcc_scan_args* a, hipStream_t st) {
     const int block = scan_block(f.per);
     f.blocks_per_group = (int)ceil_div(f.per, block);
     const int64_t grid = (int64_t)f.groups * f.blocks_per_group * f.n_chunks;
-    if (grid > 0x7fffff || (a->d_final && a->n_seqs > 0x3fffff)) return mfcc_detail::fail(MFCC_E_UNSUPPORTED, "batch too large: split it");
+    if (grid > 0x7fffff || (a->d_final && a->n_seqs > 0x3fffff)) return too_large();
+    if (f.n_chunks > 1 && (grid * sum_slices(f.state, false) > 0x7fffff || carry_blocks(f) > 0x3fffff)) return too_large();
     if (a->rows > 0) {
         const int rc = by_state(a->state, [&](auto np) {
             constexpr int NP = decltype(np)::value;
             if (f.n_chunks > 1) {
-                if (grid * sum_slices(f.state, false) > 0x7fffff) return mfcc_detail::fail(MFCC_E_UNSUPPORTED, "batch too large: split it");
                 hipLaunchKernelGGL((k_scan_sum<T, std::min(NP, sum_states(false)), false>), dim3((unsigned)(grid * sum_slices(f.state, false))),
                                    dim3(block), 0, st, f);
                 launch_carry<T>(f, 1, st);
@@ -1042,25 +1046,10 @@ int scan_backward(const mfcc_scan_args* a, hipStream_t st) {
     Scan f = scan_args(a, true);
     return by_state(a->state, [&](auto np) {
         constexpr int NP = decltype(np)::value;
-        if (a->rows > 0) {
-            const int block = scan_block(f.per);
-            f.blocks_per_group = (int)ceil_div(f.per, block);
-            const int64_t grid = (int64_t)f.groups * f.blocks_per_group * f.n_chunks;
-            if (f.n_chunks > 1) {
-                if (grid * sum_slices(f.state, true) > 0x7fffff) return mfcc_detail::fail(MFCC_E_UNSUPPORTED, "batch too large: split it");
-                hipLaunchKernelGGL((k_scan_sum<T, std::min(NP, sum_states(true)), true>), dim3((unsigned)(grid * sum_slices(f.state, true))),
-                                   dim3(block), 0, st, f);
-                launch_carry<T>(f, 2, st);
-            }
-            f.blocks_per_group = (int)ceil_div(f.per, bwd_channels<NP>());
-            const int64_t grid2 = (int64_t)f.groups * f.blocks_per_group * f.n_chunks;
-            if (grid2 > 0x7fffff) return mfcc_detail::fail(MFCC_E_UNSUPPORTED, "batch too large: split it");
-            // chunks of up to sixteen rows in a kernel with LDS and registers for as many: more workgroups per CU
-            // (the gradients of 1187 x 518 x 13 in float32 61 -> 53 us)
-            if (f.chunk <= 16) hipLaunchKernelGGL((k_scan_bwd<T, NP, 16>), dim3((unsigned)grid2), dim3(256), 0, st, f);
-            else hipLaunchKernelGGL((k_scan_bwd<T, NP, bwd_rows<NP>()>), dim3((unsigned)grid2), dim3(256), 0, st, f);
-            PACKED_LAUNCHED();
-        }
+        const int block = scan_block(f.per), sum_blocks_per_group = (int)ceil_div(f.per, block);
+        const int64_t sum_grid = (int64_t)f.groups * sum_blocks_per_group * f.n_chunks * sum_slices(f.state, true);
+        f.blocks_per_group = (int)ceil_div(f.per, bwd_channels<NP>());
+        const int64_t grid = (int64_t)f.groups * f.blocks_per_group * f.n_chunks;
         const int64_t m = a->rows * f.groups * NP;
         ReduceJobs jobs = {};
         int64_t blocks = 0;
@@ -1076,7 +1065,21 @@ int scan_backward(const mfcc_scan_args* a, hipStream_t st) {
         reduce(f.part_bias, f.n_chunks, f.channels, 1, 1, a->d_ddelta_bias, true);
         jobs.sum_blocks = blocks;
         blocks += scan_empties(a, a->d_dfinal, a->d_dinitial, &jobs.empties);
-        if (blocks > 0x1fffff) return mfcc_detail::fail(MFCC_E_UNSUPPORTED, "batch too large: split it");
+        if (grid > 0x7fffff || blocks > 0x1fffff) return too_large();
+        if (f.n_chunks > 1 && (sum_grid > 0x7fffff || carry_blocks(f) > 0x3fffff)) return too_large();
+        if (f.n_chunks > 1) {
+            Scan g = f;
+            g.blocks_per_group = sum_blocks_per_group;
+            hipLaunchKernelGGL((k_scan_sum<T, std::min(NP, sum_states(true)), true>), dim3((unsigned)sum_grid), dim3(block), 0, st, g);
+            launch_carry<T>(f, 2, st);
+        }
+        if (a->rows > 0) {
+            // chunks of up to sixteen rows in a kernel with LDS and registers for as many: more workgroups per CU
+            // (the gradients of 1187 x 518 x 13 in float32 61 -> 53 us)
+            if (f.chunk <= 16) hipLaunchKernelGGL((k_scan_bwd<T, NP, 16>), dim3((unsigned)grid), dim3(256), 0, st, f);
+            else hipLaunchKernelGGL((k_scan_bwd<T, NP, bwd_rows<NP>()>), dim3((unsigned)grid), dim3(256), 0, st, f);
+            PACKED_LAUNCHED();
+        }
         hipLaunchKernelGGL(k_scan_reduce<T>, dim3((unsigned)blocks), dim3(1024), 0, st, jobs);
         PACKED_LAUNCHED();
         return (int)MFCC_OK;

@@ -104,6 +104,26 @@ def test_workspaces_are_checked():
     assert lib.mfcc_add_norm_backward(a, None) == _lib.MFCC_E_WORKSPACE
 
 
+def test_what_a_launch_cannot_number_is_refused_before_any():
+    """Each size is one that a later launch of the call would refuse; nothing is launched before (that would end in
+    another error here, without a GPU)."""
+    lib = _lib.lib()
+    scan = dict(d_u=16, d_delta=16, d_B=16, d_C=16, d_y=16, d_dy=16, d_du=16, d_ddelta=16, d_dB=16, d_dC=16, d_dA=16,
+                d_workspace=256, workspace_bytes=2 ** 62)
+    many = 17 * 2 ** 17
+    for kw in (dict(rows=64, channels=many, groups=many),               # the sums of dB and dC
+               dict(rows=64 * 600000, channels=256, state=64),          # the gradient kernel itself
+               dict(rows=300, channels=2 ** 24, state=64)):             # the states between chunks
+        assert lib.mfcc_selective_scan_backward(scan_args(**scan, **kw), None) == _lib.MFCC_E_UNSUPPORTED, kw
+    for kw in (dict(rows=300, channels=2 ** 24, state=64), dict(rows=2 ** 33, channels=8)):
+        assert lib.mfcc_selective_scan(scan_args(**scan, **kw), None) == _lib.MFCC_E_UNSUPPORTED, kw
+    a = conv_args(rows=4, channels=2 ** 24, width=8, d_x=16, d_dy=16, d_dx=16, d_dweight=16, d_workspace=256, workspace_bytes=2 ** 62)
+    assert lib.mfcc_causal_conv_backward(a, None) == _lib.MFCC_E_UNSUPPORTED
+    a = norm_args(rows=1, channels=65535 * 32768, groups=65535, d_x=16, d_z=16, d_dy=16, d_dx=16, d_dz=16, d_dweight=16,
+                  d_workspace=256, workspace_bytes=2 ** 62)
+    assert lib.mfcc_gate_norm_backward(a, None) == _lib.MFCC_E_UNSUPPORTED
+
+
 @pytest.mark.parametrize("kw,code", [
     (dict(struct_size=8), -1), (dict(dtype=4), -1), (dict(channels=0), -1), (dict(groups=3), -1), (dict(groups=0), -1),
     (dict(channels=32769), -2), (dict(norm=2), -1), (dict(eps=0.0), -1), (dict(eps=float("nan")), -1), (dict(rows=-1), -1), (dict(rows=3), -1),
