@@ -277,6 +277,7 @@ __global__ __launch_bounds__(256) void k_scan_sum(const Scan a) {
 template <typename T, int BATCH>
 __global__ __launch_bounds__(1024) void k_scan_carry(const Scan a) {
     __shared__ float sD[16][64], sH[16][64];
+    __shared__ int s_cut[16];
     const int lane = threadIdx.x & 63, seg = threadIdx.x >> 6;
     const bool right = blockIdx.y == 1;
     float* st = right ? a.gst : a.hst;
@@ -301,20 +302,23 @@ __global__ __launch_bounds__(1024) void k_scan_carry(const Scan a) {
         for (int j = 0; j < BATCH; ++j) dec[j] = exp2_hw(A2 * dec[j]);
     };
     float D = 1.0f, H = 0.0f;
+    int any_cut = 0;
     for (int i0 = k0; i0 < k1; i0 += BATCH) {
         fetch(i0);
 #pragma unroll
         for (int j = 0; j < BATCH; ++j)
             if (i0 + j < k1) {
                 H = cut[j] ? v[j] : fmaf(dec[j], H, v[j]);
-                D = cut[j] ? 0.0f : D * dec[j];
+                D *= dec[j];
+                any_cut |= cut[j];
             }
     }
     sD[seg][lane] = D; sH[seg][lane] = H;
+    if (lane == 0) s_cut[seg] = any_cut;                   // the same for all columns
     __syncthreads();
     float carry = 0.0f;
-    // D == 0 also where a chunk of the segment is cut: nothing passes, whatever the carry is
-    for (int s = 0; s < seg; ++s) carry = sD[s][lane] == 0.0f ? sH[s][lane] : fmaf(sD[s][lane], carry, sH[s][lane]);
+    // what comes before a cut does not pass it; what comes before decays whose product is zero does, if it is a NaN
+    for (int s = 0; s < seg; ++s) carry = s_cut[s] ? sH[s][lane] : fmaf(sD[s][lane], carry, sH[s][lane]);
     for (int i0 = k0; i0 < k1; i0 += BATCH) {
         if (len > BATCH) fetch(i0);                    // a shorter segment is still in registers
 #pragma unroll
