@@ -19,10 +19,16 @@
 
 namespace packed {
 
-constexpr float SCAN_LOG2E = LOG2E;
 constexpr int SCAN_TILE = 32;       // rows of B and C staged in LDS at a time (forward kernels)
 constexpr int ZERO_ROW = SCAN_TILE;  // behind them one of zeros, for the missing rows of a group of four: with a step
                                      // of zero as well they change nothing, also behind an infinite row
+
+// A log2(e), so that a decay is exp2(d rate) and a step of zero (a missing row too) decays by one whatever the rate: a
+// product beyond the range of float32 becomes the largest number.
+__device__ __forceinline__ float rate_of(float A) {
+    const float r = A * LOG2E;
+    return fabsf(r) > 3.40282347e38f ? copysignf(3.40282347e38f, r) : r;
+}
 
 // Holds the LDS reads of the next row back until half of this row's states are done: hoisted by the compiler,
 // the B and C of four rows take the registers of two wavefronts.
@@ -152,7 +158,7 @@ __device__ __forceinline__ void store_state(float* to, const float (&v)[NP], con
 template <int NP>
 __device__ __forceinline__ void load_rates(float (&A2)[NP], const Scan& a, int c, int n0) {
 #pragma unroll
-    for (int n = 0; n < NP; ++n) A2[n] = n0 + n < a.state ? a.A[(int64_t)c * a.state + n0 + n] * SCAN_LOG2E : 0.0f;
+    for (int n = 0; n < NP; ++n) A2[n] = n0 + n < a.state ? rate_of(a.A[(int64_t)c * a.state + n0 + n]) : 0.0f;
 }
 
 // Pass 1.  A lane holds a channel and up to sixteen of its states (they are independent here: more of them are
@@ -285,7 +291,7 @@ __global__ __launch_bounds__(1024) void k_scan_carry(const Scan a) {
     const int64_t e = (int64_t)blockIdx.x * 64 + lane;
     const bool live = e < m;
     const int n = live ? (int)(e / a.channels) : 0, c = live ? (int)(e % a.channels) : 0;
-    const float A2 = a.A[(int64_t)c * a.state + n] * SCAN_LOG2E;
+    const float A2 = rate_of(a.A[(int64_t)c * a.state + n]);
     const int len = (a.n_chunks + 15) / 16;
     const int k0 = min(seg * len, a.n_chunks), k1 = min(k0 + len, a.n_chunks);
     float v[BATCH], dec[BATCH];
@@ -582,7 +588,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(bwd_waves<T
     float A2[4], h[4], G[4], dA[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        A2[i] = n0 + i < a.state ? a.A[(int64_t)c * a.state + n0 + i] * SCAN_LOG2E : 0.0f;
+        A2[i] = n0 + i < a.state ? rate_of(a.A[(int64_t)c * a.state + n0 + i]) : 0.0f;
         const bool has = a.n_chunks > 1 && live && n0 + i < a.state;
         const int64_t at = ((int64_t)k * a.state + n0 + i) * a.channels + c;
         h[i] = has ? a.hst[at] : 0.0f;
@@ -870,7 +876,7 @@ __global__ __launch_bounds__(256) void k_scan_step(const ScanStep a) {
     const float bias = a.bias ? a.bias[c] : 0.0f, skip = a.D ? a.D[c] : 0.0f;
     if (a.slots) slot_use<NE>(skipped, again, a.slots, a.batch, e0, slot);
 #pragma unroll
-    for (int n = 0; n < 4; ++n) A2[n] *= SCAN_LOG2E;
+    for (int n = 0; n < 4; ++n) A2[n] = rate_of(A2[n]);
     M* y = static_cast<M*>(a.y) + c;
     auto advance = [&](int k, int e) {
         d[k] = step_of(a.softplus, raw[k], bias);

@@ -5,7 +5,8 @@ import numpy as np
 import pytest
 import torch
 
-from tests.test_gpu_sequence import gen, randn
+from tests import sequence_ref as R
+from tests.test_gpu_sequence import F32, device_offsets, gen, rand, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -63,3 +64,37 @@ def test_nan_stays_to_the_end_of_its_sequence(gpu):
     for got, want in ((g2.u, grads.u), (g2.delta, grads.delta)):
         assert torch.isnan(got[:end - 9, at]).all()
         assert torch.equal(got[:, rest], want[:, rest]) and torch.equal(got[end - 9:], want[end - 9:])
+
+
+@pytest.mark.parametrize("rate", [-3e38, float("-inf")])
+def test_states_that_forget_at_once(gpu, rate):
+    """A rate whose product with log2 e is infinite: the state is the row's own d u B, in sequences that start and end
+    anywhere; a step of zero leaves it alone where the rate is finite."""
+    import speech_to_text_amd as S
+
+    g = gen(gpu, 2)
+    lengths, ch, n = [5, 60, 1, 45], 9, 4
+    off, rows = device_offsets(lengths, gpu), sum(lengths)
+    u, dy = randn(g, rows, ch), randn(g, rows, ch)
+    delta, B, C = rand(g, rows, ch, lo=0.01, hi=0.1), randn(g, rows, n), randn(g, rows, n)
+    A = -rand(g, ch, n, lo=0.1, hi=1.0)
+    A[:, 1] = rate
+    y, state = S.selective_scan(u, delta, A, B, C, None, None, off, return_state=True)
+    ru, rd, rA, rB, rC = R.leaves(u, delta, A, B[:, None], C[:, None], grad=False)
+    want, final = R.selective_scan(ru, rd, rA, rB, rC, offsets=off.tolist())
+    size, size_final = R.selective_scan(ru.abs(), rd, rA, rB.abs(), rC.abs(), offsets=off.tolist())
+    R.assert_close(y, want, F32, size, R.scan_steps(lengths) + n, "y")
+    R.assert_close(state, final, F32, size_final, R.scan_steps(lengths), "state")
+    got = S.selective_scan_backward(dy, u, delta, A, B, C, None, None, off)
+    assert all(torch.isfinite(t).all() for t in got if t is not None)
+    assert (got.A[:, 1] == 0).all()
+    pool = torch.ones(rows, ch, n, device=gpu)
+    S.selective_scan_step(u, delta, A, B, C, pool)
+    own = (rd * ru)[..., None] * rB
+    R.assert_close(pool[..., 1], own[..., 1], F32, own[..., 1].abs(), 2, "token")
+    if rate > float("-inf"):
+        zero = torch.zeros_like(delta)
+        init = torch.ones(len(lengths), ch, n, device=gpu)
+        _, state = S.selective_scan(u, zero, A, B, C, None, None, off, initial_state=init, return_state=True)
+        assert torch.equal(state, init)
+        S.selective_scan_step(u, zero, A, B, C, pool, new_state=torch.empty_like(pool))
