@@ -16,6 +16,8 @@ Common to all of them:
   gradients; what they hold is not looked at;
 * calls run on the current stream of the tensors' device; the same call gives the same bits;
 * arguments that do not fit raise :class:`ParameterError`;
+* what a call writes into the caller's tensors (``out``, the states of single-token calls) counts as an in-place
+  operation of torch: their version counters go up, and tensors that require a gradient are not written;
 * with gradients enabled and a differentiable input, the result has a ``grad_fn``.  Such a call cannot be
   made while a graph is captured (autograd may tie the capture to another stream): capture the plain call
   and the ``*_backward`` function under ``torch.no_grad()`` instead.
@@ -153,11 +155,19 @@ def _out(out, x, inputs, dtype=None):
     if out is None:
         return x.new_empty(x.shape, dtype=dtype or x.dtype)
     _rows(out, "out", x, dtype)
+    if out.requires_grad and torch.is_grad_enabled():
+        raise ParameterError("out requires a gradient: the call would overwrite it unseen")
     if out.shape[0] > 1 and out.stride(0) < out.shape[1]:
         raise ParameterError("the rows of out overlap")
     if any(_overlap(out, t) for t in inputs):
         raise ParameterError("out overlaps an input")
     return out
+
+
+def _wrote(*tensors):
+    """Raises the version counters of the caller's tensors that a call wrote through their pointers (None: no tensor), so
+    that a backward pass that needs what they held says so, as after torch's own in-place operations."""
+    torch.autograd.graph.increment_version([t for t in tensors if t is not None])
 
 
 def _device_offsets(frame_offsets, x):
@@ -260,6 +270,8 @@ def _conv_forward(x, weight, bias, frame_offsets, activation, initial_state, ret
         state = _new(x, (n_seqs, width - 1, x.shape[1]))
         a.d_state = state.data_ptr()
     _run(x, _lib.lib().mfcc_causal_conv, a)
+    if out is not None:
+        _wrote(out)
     return y, state
 
 
@@ -344,7 +356,7 @@ def causal_conv_step(x, state, weight, bias=None, *, activation=None, slots=None
     tensor; slot e without it), whose state after the token replaces it -- or is written to the same slot of
     ``new_state``, the others being left alone.  Rows that name one slot are successive tokens of it, in
     their order; a slot outside the pool (a padded row) gives a zero row.  Returns y."""
-    _no_grad_step(x, state, weight, bias)
+    _no_grad_step(x, state, weight, bias, new_state)
     x = _rows(x, "x")
     batch, channels = x.shape
     if not isinstance(weight, torch.Tensor) or weight.ndim != 2 or not 1 <= weight.shape[1] <= 8:
@@ -358,12 +370,13 @@ def causal_conv_step(x, state, weight, bias=None, *, activation=None, slots=None
     if state is None:
         raise ParameterError("state is missing")
     state = _state(state, "state", (n_slots, width - 1, channels), x.dtype, x, writable=True)
-    new_state = _next_state(state, _state(new_state, "new_state", (n_slots, width - 1, channels), x.dtype, x, writable=True))
+    into = _next_state(state, _state(new_state, "new_state", (n_slots, width - 1, channels), x.dtype, x, writable=True))
     slots = _slots(slots, batch, x)
-    y = _out(out, x, (x, _flat(state), _flat(new_state)) if out is not None else ())
+    y = _out(out, x, (x, _flat(state), _flat(into)) if out is not None else ())
     _run(x, _lib.lib().mfcc_causal_conv_step, _DTYPE[x.dtype], batch, n_slots, channels, width, _ACTIVATION[activation],
-         x.data_ptr(), x.stride(0), state.data_ptr(), new_state.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(slots),
+         x.data_ptr(), x.stride(0), state.data_ptr(), into.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(slots),
          y.data_ptr(), y.stride(0))
+    _wrote(into, new_state, out)
     return y
 
 
@@ -418,6 +431,8 @@ def _scan_forward(u, delta, A, B, Cm, D, delta_bias, frame_offsets, softplus, in
     ws = _workspace(_lib.lib().mfcc_selective_scan_workspace(a), u)
     a.d_workspace, a.workspace_bytes = _ptr(ws), 0 if ws is None else ws.numel()
     _run(u, _lib.lib().mfcc_selective_scan, a)
+    if out is not None:
+        _wrote(out)
     return y, final
 
 
@@ -486,7 +501,7 @@ def selective_scan_step(u, delta, A, B, C, state, D=None, delta_bias=None, *, so
     """One token of :func:`selective_scan` for each row of ``u`` (batch, channels).  ``state`` (slots, channels,
     state) float32 holds the sequences' states; ``slots``, ``new_state`` and padded rows are as in
     :func:`causal_conv_step`.  Returns y."""
-    _no_grad_step(u, delta, A, B, C, state, D, delta_bias)
+    _no_grad_step(u, delta, A, B, C, state, D, delta_bias, new_state)
     u = _rows(u, "u")
     a, keep, n_state = _scan_args(u, delta, A, B, C, D, delta_bias, softplus, 0, None)
     if state is None:
@@ -494,12 +509,13 @@ def selective_scan_step(u, delta, A, B, C, state, D=None, delta_bias=None, *, so
     n_slots = state.shape[0] if isinstance(state, torch.Tensor) and state.ndim == 3 else -1
     shape = (n_slots, u.shape[1], n_state)
     state = _state(state, "state", shape, torch.float32, u, writable=True)
-    new_state = _next_state(state, _state(new_state, "new_state", shape, torch.float32, u, writable=True))
+    into = _next_state(state, _state(new_state, "new_state", shape, torch.float32, u, writable=True))
     slots = _slots(slots, u.shape[0], u)
-    y = _out(out, u, (u, delta, B.flatten(1), C.flatten(1), _flat(state), _flat(new_state)) if out is not None else ())
-    a.d_initial, a.d_final = state.data_ptr(), new_state.data_ptr()
+    y = _out(out, u, (u, delta, B.flatten(1), C.flatten(1), _flat(state), _flat(into)) if out is not None else ())
+    a.d_initial, a.d_final = state.data_ptr(), into.data_ptr()
     a.d_y, a.y_stride = y.data_ptr(), y.stride(0)
     _run(u, _lib.lib().mfcc_selective_scan_step, a, n_slots, _ptr(slots))
+    _wrote(into, new_state, out)
     return y
 
 
@@ -655,6 +671,8 @@ def _gate_norm_forward(x, z, weight, bias, norm, groups, gate_first, eps, out):
     a.d_x, a.x_stride, a.d_z, a.z_stride = x.data_ptr(), x.stride(0), z.data_ptr(), z.stride(0)
     a.d_y, a.y_stride = y.data_ptr(), y.stride(0)
     _run(x, _lib.lib().mfcc_gate_norm, a)
+    if out is not None:
+        _wrote(out)
     return y
 
 

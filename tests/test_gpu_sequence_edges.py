@@ -98,3 +98,52 @@ def test_states_that_forget_at_once(gpu, rate):
         _, state = S.selective_scan(u, zero, A, B, C, None, None, off, initial_state=init, return_state=True)
         assert torch.equal(state, init)
         S.selective_scan_step(u, zero, A, B, C, pool, new_state=torch.empty_like(pool))
+
+
+# ---- what autograd sees -------------------------------------------------------------------------------------------
+def test_writes_raise_the_version_counter(gpu):
+    """Pools and `out` are written as by torch's own in-place operations: a tensor that a backward pass still needs is
+    missed there, and a leaf that requires a gradient is not written."""
+    import speech_to_text_amd as S
+
+    g = gen(gpu, 3)
+    ch, n, m = 6, 3, 4
+    x, w, A = randn(g, m, ch), randn(g, ch, 3), -rand(g, ch, n)
+    B = randn(g, m, n)
+    conv, scan = randn(g, m, 2, ch), randn(g, m, ch, n)
+    out, into = torch.empty_like(x), torch.empty_like(conv)
+    writes = [
+        (lambda: S.causal_conv_step(x, conv, w), [conv], [x, w, out]),
+        (lambda: S.causal_conv_step(x, conv, w, new_state=into, out=out), [into, out], [conv, x, w]),
+        (lambda: S.selective_scan_step(x, x, A, B, B, scan), [scan], [x, A, B]),
+        (lambda: S.selective_scan_step(x, x, A, B, B, scan, out=out), [scan, out], [x, A, B]),
+        (lambda: S.causal_conv(x, w, out=out), [out], [x, w]), (lambda: S.selective_scan(x, x, A, B, B, out=out), [out], [x, A, B]),
+        (lambda: S.gate_norm(x, x, out=out), [out], [x]),
+    ]
+    for i, (call, written, read) in enumerate(writes):
+        before = [t._version for t in written], [t._version for t in read]
+        call()
+        assert all(t._version > v for t, v in zip(written, before[0])), i
+        assert all(t._version == v for t, v in zip(read, before[1])), i
+    leaf = x.clone().requires_grad_()
+    for pool, f, step in ((conv, lambda p: S.causal_conv(leaf, w, None, [0, 1, 2, 3, 4], initial_state=p), lambda p: S.causal_conv_step(x, p, w)),
+                          (scan, lambda p: S.selective_scan(leaf, x, A, B, B, None, None, [0, 1, 2, 3, 4], initial_state=p),
+                           lambda p: S.selective_scan_step(x, x, A, B, B, p))):
+        y = f(pool)
+        step(pool)                                          # before the backward pass has read it
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+    for call in (lambda t: S.causal_conv(x, w, out=t), lambda t: S.gate_norm(x, x, out=t), lambda t: S.selective_scan(x, x, A, B, B, out=t),
+                 lambda t: S.causal_conv_step(x, conv, w, out=t), lambda t: S.selective_scan_step(x, x, A, B, B, scan, out=t)):
+        with pytest.raises(S.ParameterError):
+            call(torch.empty_like(x).requires_grad_())
+        with torch.no_grad():
+            call(torch.empty_like(x).requires_grad_())
+    with pytest.raises(S.ParameterError):
+        S.causal_conv_step(x, conv, w, new_state=torch.empty_like(conv).requires_grad_())
+    with pytest.raises(S.ParameterError):
+        S.selective_scan_step(x, x, A, B, B, scan, new_state=torch.empty_like(scan).requires_grad_())
+    with torch.inference_mode():
+        pool = conv.clone()
+        S.causal_conv_step(x, pool, w)
+    S.causal_conv_step(x, pool, w)                          # tensors without a counter are written all the same
