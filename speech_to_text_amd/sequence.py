@@ -20,7 +20,9 @@ Common to all of them:
   operation of torch: their version counters go up, and tensors that require a gradient are not written;
 * with gradients enabled and a differentiable input, the result has a ``grad_fn``.  Such a call cannot be
   made while a graph is captured (autograd may tie the capture to another stream): capture the plain call
-  and the ``*_backward`` function under ``torch.no_grad()`` instead.
+  and the ``*_backward`` function under ``torch.no_grad()`` instead;
+* ``*_backward`` and single-token calls have no gradient: with gradients enabled they take no tensor that requires
+  one.  There are no derivatives in forward mode, and ``torch.jit.trace`` is refused.
 """
 from __future__ import annotations
 
@@ -29,6 +31,7 @@ from typing import NamedTuple, Optional
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -220,7 +223,18 @@ def _new(x, shape, dtype=None):
     return x.new_empty(shape, dtype=dtype or x.dtype)
 
 
+def _unseen(tensors):
+    """Refuses calls whose derivative or whose very work would be lost: tangents of forward mode, and a trace, which
+    records torch's own operations only."""
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(
+            isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise ParameterError("there are no derivatives in forward mode: take them in reverse mode")
+    if torch.jit.is_tracing():
+        raise ParameterError("a call cannot be traced by torch.jit")
+
+
 def _differentiable(out, *tensors) -> bool:
+    _unseen(tensors)
     if not torch.is_grad_enabled() or not any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
         return False
     if torch.cuda.is_current_stream_capturing():
@@ -311,6 +325,7 @@ def causal_conv(x, weight, bias=None, frame_offsets=None, *, activation=None, in
 def causal_conv_backward(dy, x, weight, bias=None, frame_offsets=None, *, activation=None, initial_state=None, dstate=None):
     """Gradients of :func:`causal_conv` for the gradient ``dy`` of its rows and, or None, ``dstate`` of the
     state it returned.  ``bias`` and ``initial_state`` have gradients where they are given."""
+    _no_second_derivative(dy, x, weight, bias, initial_state, dstate)
     a, x, keep, n_seqs, width = _conv_args(x, weight, bias, frame_offsets, activation, initial_state)
     dy = _rows(dy, "dy", x)
     channels = x.shape[1]
@@ -337,8 +352,15 @@ def _slots(slots, batch, x):
 
 
 def _no_grad_step(*tensors):
+    _unseen(tensors)
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
         raise ParameterError("single-token calls have no gradient: call them under torch.no_grad()")
+
+
+def _no_second_derivative(*tensors):
+    _unseen(tensors)
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
+        raise ParameterError("explicit gradients have no gradient of their own: call them under torch.no_grad()")
 
 
 def _next_state(state, new_state):
@@ -474,6 +496,7 @@ def selective_scan_backward(dy, u, delta, A, B, C, D=None, delta_bias=None, fram
                             initial_state=None, dstate=None):
     """Gradients of :func:`selective_scan` for the gradient ``dy`` of its rows and, or None, ``dstate`` of the
     state it returned.  The states are recomputed; optional inputs have gradients where they are given."""
+    _no_second_derivative(dy, u, delta, A, B, C, D, delta_bias, initial_state, dstate)
     u = _rows(u, "u")
     off, n_seqs, keep_off = _offsets(frame_offsets, u)
     a, keep, state = _scan_args(u, delta, A, B, C, D, delta_bias, softplus, n_seqs, off)
@@ -607,6 +630,7 @@ def add_norm_backward(dy, dr, r, weight=None, bias=None, *, x=None, scale=None, 
     results (one of them may be None).  ``x`` is needed for the gradient of a learned ``scale`` only;
     ``dtype`` is x's type where ``dy`` does not tell it.  Without a scale and with one type the gradients of x
     and of the residual are the same numbers and are returned as one tensor."""
+    _no_second_derivative(dy, dr, r, weight, bias, x, scale)
     r = _rows(r, "r")
     dtype = dy.dtype if dy is not None else dtype or (x.dtype if x is not None else r.dtype)
     if dtype not in _DTYPE or r.dtype not in (dtype, torch.float32):
@@ -687,6 +711,7 @@ def gate_norm(x, z, weight=None, bias=None, *, norm="rms", groups=1, gate_first=
 
 def gate_norm_backward(dy, x, z, weight=None, bias=None, *, norm="rms", groups=1, gate_first=True, eps=1e-5):
     """Gradients of :func:`gate_norm` for the gradient ``dy`` of its result."""
+    _no_second_derivative(dy, x, z, weight, bias)
     x = _rows(x, "x")
     z = _rows(z, "z", x)
     dy = _rows(dy, "dy", x)

@@ -166,6 +166,55 @@ def test_host_tensors_are_refused():
             call()
 
 
+def all_calls(x, w, A, v, state, pool):
+    return [
+        lambda: S.causal_conv(x, w), lambda: S.causal_conv_backward(x, x, w), lambda: S.causal_conv_step(x, state, w),
+        lambda: S.selective_scan(x, x, A, v, v), lambda: S.selective_scan_backward(x, x, x, A, v, v),
+        lambda: S.selective_scan_step(x, x, A, v, v, pool), lambda: S.add_norm(x, weight=A[:, 0]),
+        lambda: S.add_norm_backward(x, None, x, A[:, 0]), lambda: S.gate_norm(x, x, A[:, 0]), lambda: S.gate_norm_backward(x, x, x, A[:, 0])]
+
+
+@pytest.mark.parametrize("which", ["x", "table"])
+def test_forward_mode_is_refused(which):
+    """A tangent would be dropped: said before anything else is looked at.  Tensors without one pass this check inside
+    a level as well."""
+    fwd = torch.autograd.forward_ad
+    x, w, A, v = torch.zeros(4, 6), torch.zeros(6, 4), torch.zeros(6, 3), torch.zeros(4, 3)
+    state, pool = torch.zeros(4, 3, 6), torch.zeros(4, 6, 3)
+    with fwd.dual_level():
+        for call in all_calls(x, w, A, v, state, pool):
+            with pytest.raises(S.ParameterError, match="device tensor"):
+                call()
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))
+        if which == "x":
+            x = dual(x)
+        else:
+            w, A = dual(w), dual(A)
+        for call in all_calls(x, w, A, v, state, pool):
+            with torch.no_grad(), pytest.raises(S.ParameterError, match="forward mode"):
+                call()
+
+
+def test_traces_are_refused():
+    x, w, A, v = torch.zeros(4, 6), torch.zeros(6, 4), torch.zeros(6, 3), torch.zeros(4, 3)
+    for i in range(10):
+        calls = lambda x: all_calls(x, w, A, v, torch.zeros(4, 3, 6), torch.zeros(4, 6, 3))
+        with pytest.raises(S.ParameterError, match="traced"):
+            torch.jit.trace(lambda x: calls(x)[i](), (x,))
+
+
+def test_explicit_gradients_have_none_of_their_own():
+    x, w, A, v = torch.zeros(4, 6), torch.zeros(6, 4), torch.zeros(6, 3), torch.zeros(4, 3)
+    backward = [1, 4, 7, 9]
+    for leaves in ((x.clone().requires_grad_(), w, A), (x, w.clone().requires_grad_(), A.clone().requires_grad_())):
+        calls = all_calls(*leaves, v, torch.zeros(4, 3, 6), torch.zeros(4, 6, 3))
+        for i in backward:
+            with pytest.raises(S.ParameterError, match="no gradient of their own"):
+                calls[i]()
+            with torch.no_grad(), pytest.raises(S.ParameterError, match="device tensor"):
+                calls[i]()
+
+
 def test_references_against_differences():
     """The 64-bit definitions the GPU tests differentiate: autograd of them against central differences."""
     g = torch.Generator().manual_seed(1)
