@@ -156,7 +156,7 @@ def _flat(t):
 def _out(out, x, inputs, dtype=None):
     """The output rows: new ones, or the caller's after a check."""
     if out is None:
-        return x.new_empty(x.shape, dtype=dtype or x.dtype)
+        return _like(x, dtype)
     _rows(out, "out", x, dtype)
     if out.requires_grad and torch.is_grad_enabled():
         raise ParameterError("out requires a gradient: the call would overwrite it unseen")
@@ -170,7 +170,9 @@ def _out(out, x, inputs, dtype=None):
 def _wrote(*tensors):
     """Raises the version counters of the caller's tensors that a call wrote through their pointers (None: no tensor), so
     that a backward pass that needs what they held says so, as after torch's own in-place operations."""
-    torch.autograd.graph.increment_version([t for t in tensors if t is not None])
+    for t in tensors:
+        if t is not None:
+            torch.autograd.graph.increment_version(t)
 
 
 def _device_offsets(frame_offsets, x):
@@ -216,6 +218,11 @@ def _run(x, fn, *args):
 
 def _workspace(size, x):
     return x.new_empty(size, dtype=torch.uint8) if size else None
+
+
+def _like(t, dtype=None):
+    """An uninitialised contiguous tensor of t's shape (1.2 us; new_empty 1.9 us)."""
+    return torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)
 
 
 def _new(x, shape, dtype=None):
@@ -330,7 +337,7 @@ def causal_conv_backward(dy, x, weight, bias=None, frame_offsets=None, *, activa
     dy = _rows(dy, "dy", x)
     channels = x.shape[1]
     dstate = _state(dstate, "dstate", (n_seqs, width - 1, channels), x.dtype, x)
-    dx = _new(x, x.shape)
+    dx = _like(x)
     dweight = _new(x, (channels, width), torch.float32)
     dbias = None if bias is None else _new(x, (channels,), torch.float32)
     dinitial = None if initial_state is None else _new(x, (n_seqs, width - 1, channels))
@@ -398,7 +405,7 @@ def causal_conv_step(x, state, weight, bias=None, *, activation=None, slots=None
     _run(x, _lib.lib().mfcc_causal_conv_step, _DTYPE[x.dtype], batch, n_slots, channels, width, _ACTIVATION[activation],
          x.data_ptr(), x.stride(0), state.data_ptr(), into.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(slots),
          y.data_ptr(), y.stride(0))
-    _wrote(into, new_state, out)
+    _wrote(into, None if new_state is into else new_state, out)
     return y
 
 
@@ -506,7 +513,7 @@ def selective_scan_backward(dy, u, delta, A, B, C, D=None, delta_bias=None, fram
     dstate = _state(dstate, "dstate", shape, torch.float32, u)
 
     def new(like, dtype):
-        return None if like is None else _new(u, like.shape, dtype)
+        return None if like is None else _like(like, dtype)
 
     f32 = torch.float32
     g = ScanGradients(new(u, u.dtype), new(u, u.dtype), new(A, f32), new(B, u.dtype), new(C, u.dtype), new(D, f32),
@@ -538,7 +545,7 @@ def selective_scan_step(u, delta, A, B, C, state, D=None, delta_bias=None, *, so
     a.d_initial, a.d_final = state.data_ptr(), into.data_ptr()
     a.d_y, a.y_stride = y.data_ptr(), y.stride(0)
     _run(u, _lib.lib().mfcc_selective_scan_step, a, n_slots, _ptr(slots))
-    _wrote(into, new_state, out)
+    _wrote(into, None if new_state is into else new_state, out)
     return y
 
 
@@ -580,7 +587,7 @@ def _add_norm_forward(x, residual, weight, bias, scale, norm, eps, residual_dtyp
     if residual is not None:
         residual = _rows(residual, "residual", x, rt)
     a, keep = _norm_args(x, weight, bias, scale, norm, eps, 1, False, rt)
-    y, r = _new(x, x.shape), _new(x, x.shape, rt)
+    y, r = _like(x), _like(x, rt)
     a.d_x, a.x_stride = x.data_ptr(), x.stride(0)
     if residual is not None:
         a.d_residual, a.residual_stride = residual.data_ptr(), residual.stride(0)
@@ -651,9 +658,9 @@ def add_norm_backward(dy, dr, r, weight=None, bias=None, *, x=None, scale=None, 
     def vector(like):
         return None if like is None else _new(r, (channels,), torch.float32)
 
-    dresidual = _new(r, r.shape)
+    dresidual = _like(r)
     one = r.dtype == dtype and not learned and a.scale_value == 1.0
-    dx = dresidual if one else _new(r, r.shape, dtype)
+    dx = dresidual if one else _like(r, dtype)
     g = AddNormGradients(dx, dresidual, vector(weight), vector(bias), vector(scale if learned else None))
     a.d_r, a.r_stride = r.data_ptr(), r.stride(0)
     if dy is not None:
@@ -721,7 +728,7 @@ def gate_norm_backward(dy, x, z, weight=None, bias=None, *, norm="rms", groups=1
     def vector(like):
         return None if like is None else _new(x, (channels,), torch.float32)
 
-    g = GateNormGradients(_new(x, x.shape), _new(x, x.shape), vector(weight), vector(bias))
+    g = GateNormGradients(_like(x), _like(x), vector(weight), vector(bias))
     a.d_x, a.x_stride, a.d_z, a.z_stride = x.data_ptr(), x.stride(0), z.data_ptr(), z.stride(0)
     a.d_dy, a.dy_stride = dy.data_ptr(), dy.stride(0)
     a.d_dx, a.d_dz, a.d_dweight, a.d_dbias = g.x.data_ptr(), g.z.data_ptr(), _ptr(g.weight), _ptr(g.bias)
