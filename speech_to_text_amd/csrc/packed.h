@@ -117,28 +117,30 @@ __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2
 __device__ __forceinline__ float log2_hw(float x) { return __builtin_amdgcn_logf(x); }
 __device__ __forceinline__ float rcp_hw(float x) { return __builtin_amdgcn_rcpf(x); }
 
-// exp(x): the product with log2(e) is carried in two floats, so that its rounding does not grow with |x|.
+// exp(x) = exp2(p) exp(x - p ln 2) with p the rounded x log2(e): the second factor is 1 + (x - p ln 2) within 2^-36, and
+// p ln 2 in two floats keeps the error from growing with |x| (at most two units beside exp2's own).
+constexpr float LN2_REST = -1.90465429995776804525e-9f;       // ln 2 - LN2
+__device__ __forceinline__ float exp_rest(float x, float p) { return fmaf(p, -LN2_REST, fmaf(p, -LN2, x)); }
 __device__ __forceinline__ float exp_f(float x) {
-    const float p = x * LOG2E;
-    const float lo = fmaf(x, LOG2E, -p) + x * 1.92596299e-8f;    // the rest of x * log2(e); NaN for infinite x
-    const float e = exp2_hw(p);
+    const float p = x * LOG2E, e = exp2_hw(p);
     // outside the finite, normal range the correction is meaningless (and inf * 0 or inf - inf appears in it)
-    return fabsf(p) < 126.0f ? fmaf(e * LN2, lo, e) : e;
+    return fabsf(p) < 126.0f ? fmaf(e, exp_rest(x, p), e) : e;
 }
 
-// EXACT = false leaves out the second float of the exponent's product: |x| 2^-24 more, for results or
-// arguments that are rounded to 16 bits anyway.
-template <bool EXACT = true>
-__device__ __forceinline__ float sigmoid_f(float x) {
-    return rcp_hw(1.0f + (EXACT ? exp_f(-x) : exp2_hw(x * -LOG2E)));
-}
+__device__ __forceinline__ float sigmoid_f(float x) { return rcp_hw(1.0f + exp_f(-x)); }
+
+// For a result that is rounded to 16 bits and goes nowhere else: without the second float of the exponent's product
+// the sigmoid is off by |x| 2^-24 more, below 2^-17 up to |x| = 88, where it leaves float32's range; half a step of
+// bfloat16 is 2^-9 of the value, of float16 2^-12.  Whatever has float32 results takes sigmoid_f.
+__device__ __forceinline__ float sigmoid_to_16(float x) { return rcp_hw(1.0f + exp2_hw(x * -LOG2E)); }
 
 // log(1 + exp(x)) = max(x, 0) + log(1 + e), e = exp(-|x|) in (0, 1].  w = 1 + e loses the low bits of a
 // small e; what it lost, e - (w - 1), is exact and is added back (to first order: the error of that is
 // below 2^-24 e).
-template <bool EXACT = true>
 __device__ __forceinline__ float softplus_f(float x) {
-    const float e = EXACT ? exp_f(-fabsf(x)) : exp2_hw(-fabsf(x) * LOG2E);
+    // exp_f of -|x|, which -100 does not change (its exp is below the smallest float32) but for the infinity it takes away
+    const float v = __builtin_elementwise_maximum(-fabsf(x), -100.0f);     // a NaN stays
+    const float p = v * LOG2E, e0 = exp2_hw(p), e = fmaf(e0, exp_rest(v, p), e0);
     const float w = 1.0f + e;
     return fmaxf(x, 0.0f) + fmaf(log2_hw(w), LN2, e - (w - 1.0f));
 }

@@ -88,7 +88,7 @@ __global__ __launch_bounds__(256) void k_conv_fwd(const ConvFwd a) {
     auto finish = [&](float (&acc)[VEC], int64_t row) {
         if (a.act) {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) acc[i] *= sigmoid_f<sizeof(M) == 4>(acc[i]);
+            for (int i = 0; i < VEC; ++i) acc[i] *= sizeof(M) == 4 ? sigmoid_f(acc[i]) : sigmoid_to_16(acc[i]);
         }
         store_vec<M, VEC>(y + row * a.y_stride, acc, n);
     };
@@ -252,7 +252,7 @@ __global__ __launch_bounds__(256) void k_conv_bwd(const ConvBwd a) {
                             float p = b[i];
 #pragma unroll
                             for (int j = 0; j < K; ++j) p = fmaf(w[j][i], tap[j][i], p);
-                            const float sg = sigmoid_f<sizeof(M) == 4>(p);
+                            const float sg = sigmoid_f(p);
                             d[i] *= sg * fmaf(p, 1.0f - sg, 1.0f);
                         }
                     }

@@ -209,7 +209,7 @@ void k_norm_bwd(const Norm a) {
             for (int i = 0; i < NV; ++i) {
                 const float dy = in.dy[k].get(i);
                 if (GATE) {
-                    const float z = in.z[GATE ? k : 0].get(i), x = in.x[k].get(i), gate = z * sigmoid_f<sizeof(M) == 4>(z);
+                    const float z = in.z[GATE ? k : 0].get(i), x = in.x[k].get(i), gate = z * sigmoid_f(z);
                     v[k][i] = a.gate_first ? x * gate : x;
                     dn[k][i] = (a.gate_first ? dy : dy * gate) * w[k][i];
                 } else {
@@ -263,7 +263,7 @@ void k_norm_bwd(const Norm a) {
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
                     const float z = in.z[GATE ? k : 0].get(i), x = in.x[k].get(i), dy = in.dy[k].get(i);
-                    const float sg = sigmoid_f<sizeof(M) == 4>(z), gate = z * sg, slope = sg * fmaf(z, 1.0f - sg, 1.0f);
+                    const float sg = sigmoid_f(z), gate = z * sg, slope = sg * fmaf(z, 1.0f - sg, 1.0f);
                     const float body = a.gate_first ? dy : dy * gate;
                     dz[i] = (a.gate_first ? dv[i] * x : dy * fmaf(v[k][i], w[k][i], t[k][i])) * slope;
                     if (a.gate_first) dv[i] *= gate;
@@ -349,7 +349,7 @@ struct NormColumns {
             load_or<M>(x, a.x ? static_cast<const M*>(a.x) + row * a.x_stride + c : nullptr, n, 0.0f);
         }
     }
-    __device__ __forceinline__ float gate(int i) const { return z[i] * sigmoid_f<sizeof(typename T::mem) == 4>(z[i]); }
+    __device__ __forceinline__ float gate(int i) const { return z[i] * sigmoid_f(z[i]); }
     // the value that is normalised, and the gradient of the normalised one
     __device__ __forceinline__ float value(const Norm& a, int i) const { return !GATE ? r[i] : a.gate_first ? x[i] * gate(i) : x[i]; }
     __device__ __forceinline__ float grad(const Norm& a, int i) const {
@@ -405,7 +405,7 @@ __global__ __launch_bounds__(1024) void k_norm_bwd_wide(const Norm a) {
                 const float vn = (in.value(a, i) - mean) * q;
                 dv[i] = (in.grad(a, i) - dmean - vn * proj) * q;
                 if (GATE) {
-                    const float z = in.z[i], sg = sigmoid_f<sizeof(M) == 4>(z), slope = sg * fmaf(z, 1.0f - sg, 1.0f);
+                    const float z = in.z[i], sg = sigmoid_f(z), slope = sg * fmaf(z, 1.0f - sg, 1.0f);
                     dz[i] = (a.gate_first ? dv[i] * in.x[i] : in.dy[i] * fmaf(vn, in.w[i], in.t[i])) * slope;
                     if (a.gate_first) dv[i] *= z * sg;
                 } else {

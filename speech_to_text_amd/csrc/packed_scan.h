@@ -23,8 +23,10 @@ constexpr int SCAN_TILE = 32;       // rows of B and C staged in LDS at a time (
 constexpr int ZERO_ROW = SCAN_TILE;  // behind them one of zeros, for the missing rows of a group of four: with a step
                                      // of zero as well they change nothing, also behind an infinite row
 
-// A log2(e), so that a decay is exp2(d rate) and a step of zero (a missing row too) decays by one whatever the rate: a
-// product beyond the range of float32 becomes the largest number.
+// A log2(e), so that a decay is exp2(d rate): d A is rounded twice where exp(d A) would round it once, and a decay over
+// rows with sum |d A| = X is off by up to X 2^-23 of itself.  For A <= 0 that is at most 2^-23 / e of the state (X exp(-X)
+// <= 1 / e).  A second float of the product would cost two more operations per element, of five.  Also, a step of
+// zero (a missing row too) decays by one whatever the rate: a product beyond the range of float32 becomes the largest number.
 __device__ __forceinline__ float rate_of(float A) {
     const float r = A * LOG2E;
     return fabsf(r) > 3.40282347e38f ? copysignf(3.40282347e38f, r) : r;
@@ -48,18 +50,17 @@ struct Scan {
     int n_seqs, channels, state, groups, per, chunk, n_chunks, blocks_per_group, softplus, zero_rest;
 };
 
-// d of a row.  In the 16-bit types delta itself is rounded to 2^-9 and less, so softplus takes its exponential
-// without the second float of the exponent's product (|delta| 2^-24 more).
+// d of a row.
 template <typename M>
 __device__ __forceinline__ float step_of(int softplus, M raw, float bias) {
     const float v = widen(raw) + bias;
-    return softplus ? softplus_f<sizeof(M) == 4>(v) : v;
+    return softplus ? softplus_f(v) : v;
 }
 template <int COUNT, typename M>
 __device__ __forceinline__ void steps_of(float (&d)[COUNT], int softplus, const M (&raw)[COUNT], float bias) {
     if (softplus) {                     // the branch outside: what a block knows of its values saves operations
 #pragma unroll
-        for (int j = 0; j < COUNT; ++j) d[j] = softplus_f<sizeof(M) == 4>(widen(raw[j]) + bias);
+        for (int j = 0; j < COUNT; ++j) d[j] = softplus_f(widen(raw[j]) + bias);
     } else {
 #pragma unroll
         for (int j = 0; j < COUNT; ++j) d[j] = widen(raw[j]) + bias;
@@ -768,7 +769,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(bwd_waves<T
                 v[i] = sd[(sq + i) * SD + t];
                 x[i] = widen(su[(sq + i) * SM + t]);
                 if (sflag[t] & OUT) v[i] = 0.0f;
-                else if (a.softplus) v[i] *= sigmoid_f<sizeof(M) == 4>(raw[p][i] + bias[i]);
+                else if (a.softplus) v[i] *= sigmoid_f(raw[p][i] + bias[i]);
                 db[i] += v[i];
             }
             const int64_t at = (r0 + t) * a.channels + c_base + sq;

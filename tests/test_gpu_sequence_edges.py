@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from tests import sequence_ref as R
-from tests.test_gpu_sequence import F32, device_offsets, gen, rand, randn
+from tests.test_gpu_sequence import F32, TYPES, device_offsets, gen, rand, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -147,3 +147,44 @@ def test_writes_raise_the_version_counter(gpu):
         pool = conv.clone()
         S.causal_conv_step(x, pool, w)
     S.causal_conv_step(x, pool, w)                          # tensors without a counter are written all the same
+
+
+# ---- float32 results of 16-bit rows ---------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES)
+def test_float32_results_carry_float32_functions(gpu, dtype):
+    """Far out, where an exponent rounded once more (|p| 2^-24 and more) would show: the state's softplus, the gradient
+    of its bias, and the gradients of taps, biases and norm weights through SiLU."""
+    import speech_to_text_amd as S
+
+    at = torch.tensor([-80.0, -61.25, -43.5, -20.75, -9.5, -3.25, 1.5, 7.75, 30.5])     # exact in every type
+    ch, p = len(at), at.double()
+    x, one = at[None].to(gpu, dtype), torch.ones(1, ch, dtype=dtype, device=gpu)
+    ones = torch.ones(1, 1, dtype=dtype, device=gpu)
+
+    def close(got, want, steps, size=None):
+        R.assert_close(got.flatten(), want, F32, want.abs() if size is None else size, steps)
+
+    # softplus: its exp 3 units, log 2 (near zero the exp's own), two sums; times u and B
+    zero_A = torch.zeros(ch, 1, device=gpu)
+    _, h = S.selective_scan(one, x, zero_A, ones, ones, softplus=True, return_state=True)
+    close(h, R.softplus(p), 8)
+    pool = torch.zeros(1, ch, 1, device=gpu)
+    S.selective_scan_step(one, x, zero_A, ones, ones, pool, softplus=True)
+    close(pool, R.softplus(p), 8)
+    # ddelta_bias = sigmoid(delta) here: exp 3, sum 1, reciprocal 1, product
+    zero = torch.zeros(ch, device=gpu)
+    grads = S.selective_scan_backward(one, one, x, zero_A, ones, ones, None, zero, softplus=True)
+    sig = 1 / (1 + torch.exp(-p))
+    close(grads.delta_bias, sig, 8)
+    # SiLU'(p) = sig (1 + p (1 - sig)): the sigmoid's units in both factors, and the sum's cancellation
+    slope, size = sig * (1 + p * (1 - sig)), sig * (1 + p.abs() * (1 - sig))
+    g = S.causal_conv_backward(one, x, torch.ones(ch, 1, device=gpu), zero, activation="silu")
+    close(g.bias, slope, 16, size)
+    close(g.weight, slope * p, 17, size * p.abs())
+    # (norm(x) w + b) silu(z): dbias = dy silu(z), in rows held in registers and in wide ones
+    for width in (ch, 8200):
+        z = torch.zeros(1, width, dtype=dtype, device=gpu)
+        z[:, :ch] = x
+        w = torch.ones(width, device=gpu)
+        g = S.gate_norm_backward(torch.ones_like(z), torch.ones_like(z), z, w, w, gate_first=False)
+        close(g.bias[:ch], p * sig, 8)
