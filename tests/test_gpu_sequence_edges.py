@@ -188,3 +188,17 @@ def test_float32_results_carry_float32_functions(gpu, dtype):
         w = torch.ones(width, device=gpu)
         g = S.gate_norm_backward(torch.ones_like(z), torch.ones_like(z), z, w, w, gate_first=False)
         close(g.bias[:ch], p * sig, 8)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_tokens_give_the_bits_of_the_prompt(gpu, dtype):
+    """Many values: the convolution token by token rounds as the convolution of the whole sequence does."""
+    import speech_to_text_amd as S
+
+    g = gen(gpu, 5)
+    rows, ch = 48, 8192
+    x, w, b = randn(g, rows, ch, dtype=dtype), randn(g, ch, 4), randn(g, ch)
+    whole, last = S.causal_conv(x, w, b, activation="silu", return_state=True)
+    state = torch.zeros(1, 3, ch, dtype=dtype, device=gpu)
+    tokens = S.causal_conv_step(x, state, w, b, activation="silu", slots=torch.zeros(rows, dtype=torch.int32, device=gpu))
+    assert torch.equal(tokens, whole) and torch.equal(state, last)
