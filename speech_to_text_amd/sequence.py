@@ -142,14 +142,14 @@ def _overlap(a, b) -> bool:
     if a1 <= b0 or b1 <= a0:
         return False
     step = a.stride(0) * a.element_size()
-    if step == b.stride(0) * b.element_size() and step > 0:         # column ranges of one matrix
+    if step > 0 and (step == b.stride(0) * b.element_size() or b.shape[0] == 1):         # column ranges of one matrix
         off = (b0 - a0) % step
         return not (off >= a.shape[1] * a.element_size() and off + b.shape[1] * b.element_size() <= step)
     return True
 
 
 def _flat(t):
-    """A contiguous state as rows, for the overlap check."""
+    """A contiguous state, table or list as rows, for the overlap check."""
     return None if t is None else t.reshape(1, -1)
 
 
@@ -284,7 +284,7 @@ def _conv_args(x, weight, bias, frame_offsets, activation, initial_state):
 
 def _conv_forward(x, weight, bias, frame_offsets, activation, initial_state, return_state, out):
     a, x, keep, n_seqs, width = _conv_args(x, weight, bias, frame_offsets, activation, initial_state)
-    y = _out(out, x, (x, _flat(initial_state)) if out is not None else ())
+    y = _out(out, x, (x, *map(_flat, keep)) if out is not None else ())
     a.d_y, a.y_stride, a.zero_rest = y.data_ptr(), y.stride(0), out is None
     state = None
     if return_state:
@@ -383,7 +383,7 @@ def causal_conv_step(x, state, weight, bias=None, *, activation=None, slots=None
     """One token of :func:`causal_conv` for each row of ``x`` (batch, channels).  ``state`` (slots, width - 1,
     channels) holds the sequences' last rows; row e continues the sequence in slot ``slots[e]`` (int32 device
     tensor; slot e without it), whose state after the token replaces it -- or is written to the same slot of
-    ``new_state``, the others being left alone.  Rows that name one slot are successive tokens of it, in
+    ``new_state``, the others being left alone; neither pool overlaps another argument.  Rows that name one slot are successive tokens of it, in
     their order; a slot outside the pool (a padded row) gives a zero row.  Returns y."""
     _no_grad_step(x, state, weight, bias, new_state)
     x = _rows(x, "x")
@@ -401,7 +401,7 @@ def causal_conv_step(x, state, weight, bias=None, *, activation=None, slots=None
     state = _state(state, "state", (n_slots, width - 1, channels), x.dtype, x, writable=True)
     into = _next_state(state, _state(new_state, "new_state", (n_slots, width - 1, channels), x.dtype, x, writable=True))
     slots = _slots(slots, batch, x)
-    y = _out(out, x, (x, _flat(state), _flat(into)) if out is not None else ())
+    y = _out(out, x, (x, *map(_flat, (state, into, weight, bias, slots))) if out is not None else ())
     _run(x, _lib.lib().mfcc_causal_conv_step, _DTYPE[x.dtype], batch, n_slots, channels, width, _ACTIVATION[activation],
          x.data_ptr(), x.stride(0), state.data_ptr(), into.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(slots),
          y.data_ptr(), y.stride(0))
@@ -451,7 +451,7 @@ def _scan_forward(u, delta, A, B, Cm, D, delta_bias, frame_offsets, softplus, in
     shape = (n_seqs, u.shape[1], state)
     initial_state = _state(initial_state, "initial_state", shape, torch.float32, u)
     a.d_initial = _ptr(initial_state)
-    y = _out(out, u, (u, delta, B.flatten(1), Cm.flatten(1), _flat(initial_state)) if out is not None else ())
+    y = _out(out, u, (u, delta, B.flatten(1), Cm.flatten(1), *map(_flat, (initial_state, keep_off, *keep))) if out is not None else ())
     a.d_y, a.y_stride, a.zero_rest = y.data_ptr(), y.stride(0), out is None
     final = None
     if return_state:
@@ -541,7 +541,7 @@ def selective_scan_step(u, delta, A, B, C, state, D=None, delta_bias=None, *, so
     state = _state(state, "state", shape, torch.float32, u, writable=True)
     into = _next_state(state, _state(new_state, "new_state", shape, torch.float32, u, writable=True))
     slots = _slots(slots, u.shape[0], u)
-    y = _out(out, u, (u, delta, B.flatten(1), C.flatten(1), _flat(state), _flat(into)) if out is not None else ())
+    y = _out(out, u, (u, delta, B.flatten(1), C.flatten(1), *map(_flat, (state, into, slots, *keep))) if out is not None else ())
     a.d_initial, a.d_final = state.data_ptr(), into.data_ptr()
     a.d_y, a.y_stride = y.data_ptr(), y.stride(0)
     _run(u, _lib.lib().mfcc_selective_scan_step, a, n_slots, _ptr(slots))
@@ -698,7 +698,7 @@ def _gate_norm_forward(x, z, weight, bias, norm, groups, gate_first, eps, out):
     x = _rows(x, "x")
     z = _rows(z, "z", x)
     a, keep = _norm_args(x, weight, bias, None, norm, eps, groups, gate_first, x.dtype)
-    y = _out(out, x, (x, z))
+    y = _out(out, x, (x, z, *map(_flat, keep)) if out is not None else ())
     a.d_x, a.x_stride, a.d_z, a.z_stride = x.data_ptr(), x.stride(0), z.data_ptr(), z.stride(0)
     a.d_y, a.y_stride = y.data_ptr(), y.stride(0)
     _run(x, _lib.lib().mfcc_gate_norm, a)

@@ -202,3 +202,38 @@ def test_tokens_give_the_bits_of_the_prompt(gpu, dtype):
     state = torch.zeros(1, 3, ch, dtype=dtype, device=gpu)
     tokens = S.causal_conv_step(x, state, w, b, activation="silu", slots=torch.zeros(rows, dtype=torch.int32, device=gpu))
     assert torch.equal(tokens, whole) and torch.equal(state, last)
+
+
+# ---- refusals -----------------------------------------------------------------------------------------------------------
+def test_out_over_a_table_is_refused(gpu):
+    """Tables, offsets and slots are inputs too."""
+    import speech_to_text_amd as S
+
+    ch, n, m = 6, 4, 10
+    memory = torch.zeros(200, device=gpu)
+    out = memory[40:40 + m * ch].view(m, ch)
+    x, free = torch.zeros(m, ch, device=gpu), torch.zeros(m, ch, device=gpu)
+    table = lambda *s, at=90: memory[at:at + int(np.prod(s))].view(s)
+    w, v, A, B = torch.zeros(ch, 3, device=gpu), torch.zeros(ch, device=gpu), torch.zeros(ch, n, device=gpu), torch.zeros(m, n, device=gpu)
+    off = memory[96:102].view(torch.int64)[:2]
+    slots = memory[90:100].view(torch.int32)
+    pool, states = torch.zeros(m, 2, ch, device=gpu), torch.zeros(m, ch, n, device=gpu)
+    calls = [
+        lambda o: S.causal_conv(x, table(ch, 3), out=o), lambda o: S.causal_conv(x, w, table(ch), out=o),
+        lambda o: S.causal_conv(x, w, None, off, out=o), lambda o: S.selective_scan(x, x, table(ch, n), B, B, out=o),
+        lambda o: S.selective_scan(x, x, A, B, B, table(ch), out=o), lambda o: S.selective_scan(x, x, A, B, B, None, table(ch), out=o),
+        lambda o: S.selective_scan(x, x, A, B, B, None, None, off, out=o), lambda o: S.gate_norm(x, x, table(ch), out=o),
+        lambda o: S.gate_norm(x, x, None, table(ch), out=o), lambda o: S.causal_conv_step(x, pool, table(ch, 3), out=o),
+        lambda o: S.causal_conv_step(x, pool, w, table(ch), out=o), lambda o: S.causal_conv_step(x, pool, w, slots=slots, out=o),
+        lambda o: S.selective_scan_step(x, x, table(ch, n), B, B, states, out=o),
+        lambda o: S.selective_scan_step(x, x, A, B, B, states, table(ch), out=o),
+        lambda o: S.selective_scan_step(x, x, A, B, B, states, None, table(ch), out=o),
+        lambda o: S.selective_scan_step(x, x, A, B, B, states, slots=slots, out=o),
+    ]
+    for i, call in enumerate(calls):
+        try:
+            call(out)
+        except S.ParameterError:
+            call(free)
+            continue
+        pytest.fail(f"call {i} was not refused")
