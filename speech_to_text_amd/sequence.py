@@ -383,8 +383,9 @@ def causal_conv_step(x, state, weight, bias=None, *, activation=None, slots=None
     """One token of :func:`causal_conv` for each row of ``x`` (batch, channels).  ``state`` (slots, width - 1,
     channels) holds the sequences' last rows; row e continues the sequence in slot ``slots[e]`` (int32 device
     tensor; slot e without it), whose state after the token replaces it -- or is written to the same slot of
-    ``new_state``, the others being left alone; neither pool overlaps another argument.  Rows that name one slot are successive tokens of it, in
-    their order; a slot outside the pool (a padded row) gives a zero row.  Returns y."""
+    ``new_state``, the others being left alone; neither pool overlaps another argument.  Rows that name one
+    slot are successive tokens of it, in their order; a slot outside the pool (a padded row) gives a zero
+    row.  Returns y."""
     _no_grad_step(x, state, weight, bias, new_state)
     x = _rows(x, "x")
     batch, channels = x.shape

@@ -120,3 +120,67 @@ def scan_steps(lengths):
     log2 e one each; v_exp_f32 one) with |d A| < 1 in the tests, and adds one product of four factors."""
     return 16 * (max(lengths, default=1) + 4)
 
+
+
+def scan_gradient_case(device, case, dtype, seed, scan_case):
+    """A case of a scan's gradients: (u, delta, A, B, C, D, bias), initial states, dy, the final states' gradient, offsets."""
+    lengths, tail, ch, n, groups, plus, has_D, has_bias = case
+    g, u, delta, A, B, C, D, bias = scan_case(device, *case, dtype, seed)
+    more = lambda *s: torch.randn(*s, generator=g, device=device)
+    init, dstate, dy = more(len(lengths), ch, n), more(len(lengths), ch, n), more(*u.shape).to(dtype)
+    clean = sum(lengths)
+    for t in (u, delta, B, C, dy):
+        t[clean:] = float("nan")
+    off = torch.tensor(lengths_to_offsets(lengths), dtype=torch.int64, device=device)
+    return (u, delta, A, B, C, D, bias), init, dy, dstate, off, plus, clean
+
+
+def scan_gradients(dy, u, delta, A, B, C, D, bias, off, plus, init, dstate, clean):
+    """({name: gradient}, {name: the same sums of absolute values}, {name: roundings on the longest way}) of a scan, by
+    the backward recurrence g = C dy + a g written out; the gradients themselves by autograd of the definition."""
+    u, delta, B, C, dy = (t[:clean] for t in (u, delta, B, C, dy))
+    ru, rd, rA, rB, rC, rD, rb, ri = leaves(u, delta, A, B, C, D, bias, init)
+    v = (rd if rb is None else rd + rb).detach()
+    d, slope = (softplus(v), torch.sigmoid(v)) if plus else (v, torch.ones_like(v))
+    d.requires_grad_()            # autograd of softplus's own form above is not its derivative where v is exactly zero
+    y, final = selective_scan(ru, d, rA, rB, rC, rD, None, off, False, ri)
+    dy, dstate = dy.double().cpu(), dstate.double().cpu()
+    named = dict(u=ru, delta=d, A=rA, B=rB, C=rC, D=rD, initial_state=ri)
+    named = {k: v for k, v in named.items() if v is not None}
+    refs = torch.autograd.grad((y * dy).sum() + (final * dstate).sum(), list(named.values()), allow_unused=True)
+    refs = {k: torch.zeros_like(v) if r is None else r for (k, v), r in zip(named.items(), refs)}
+    refs["delta"] = refs["delta"] * slope
+    if rb is not None:
+        refs["delta_bias"] = refs["delta"].sum(0)
+    with torch.no_grad():
+        ch, n, per = u.shape[1], A.shape[1], u.shape[1] // B.shape[1]
+        wide = lambda m, t: m[t].abs().repeat_interleave(per, 0)
+        narrow = lambda m: m.reshape(-1, per, n).sum(1)
+        ua, ya, decay = ru.abs(), dy.abs(), lambda t: torch.exp(d[t, :, None] * rA)
+        s = {k: torch.zeros_like(t) for k, t in named.items()}
+        dd = torch.zeros_like(ru)
+        for q, (lo, hi) in enumerate(zip(off[:-1], off[1:])):
+            hs = [ri[q].abs()]
+            for t in range(lo, hi):
+                hs.append(decay(t) * hs[-1] + (d[t].abs() * ua[t])[:, None] * wide(rB, t))
+            carry = dstate[q].abs()
+            for t in range(hi - 1, lo - 1, -1):
+                g = carry + ya[t, :, None] * wide(rC, t)
+                s["C"][t], s["B"][t] = narrow(ya[t, :, None] * hs[t - lo + 1]), narrow(g * (d[t].abs() * ua[t])[:, None])
+                carry = g * decay(t)
+                gB, w = (g * wide(rB, t)).sum(1), carry * hs[t - lo]
+                s["u"][t] = d[t].abs() * gB + (0 if rD is None else rD.abs() * ya[t])
+                dd[t] = ua[t] * gB + (w * rA.abs()).sum(1)
+                s["A"] += w * d[t, :, None].abs()
+            s["initial_state"][q] = carry
+        s["delta"] = dd * slope
+        if rD is not None:
+            s["D"] = (ua * ya).sum(0)
+        if rb is not None:
+            s["delta_bias"] = s["delta"].sum(0)
+    # a state, and the gradient of one, each come through at most the longest sequence's decays; then the sum over the
+    # states or the channels, the slope's functions (8), products; and the sum over rows
+    longest = max((hi - lo for lo, hi in zip(off[:-1], off[1:])), default=0)
+    way = 2 * scan_steps([longest])
+    extra = dict(u=n + 8, delta=n + 16, A=clean + 8, B=ch + 8, C=ch + 8, D=clean + 4, delta_bias=clean + n + 16, initial_state=8)
+    return refs, s, {k: way + extra[k] for k in refs}

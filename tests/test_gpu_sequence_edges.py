@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from tests import sequence_ref as R
-from tests.test_gpu_sequence import F32, TYPES, device_offsets, gen, rand, randn
+from tests.test_gpu_sequence import F32, SCAN, TYPES, device_offsets, gen, rand, randn, scan_case
 
 pytestmark = pytest.mark.gpu
 
@@ -149,6 +149,34 @@ def test_writes_raise_the_version_counter(gpu):
     S.causal_conv_step(x, pool, w)                          # tensors without a counter are written all the same
 
 
+def test_frozen_tables_and_rows(gpu):
+    """Whatever does not require a gradient gets none, and the others' are those of a call where all do."""
+    import speech_to_text_amd as S
+
+    g = gen(gpu, 6)
+    m, ch, n = 40, 12, 4
+    rows = lambda: randn(g, m, ch)
+    per = lambda *s: randn(g, ch, *s)
+    init, h0 = randn(g, 1, 2, ch), randn(g, 1, ch, n)
+    calls = [
+        (lambda x, w, b, i: S.causal_conv(x, w, b, activation="silu", initial_state=i), [rows(), per(3), per(), init]),
+        (lambda u, d, A, B, C, D, b, i: S.selective_scan(u, d, A, B, C, D, b, softplus=True, initial_state=i),
+         [rows(), rows(), -rand(g, ch, n), randn(g, m, n), randn(g, m, n), per(), per(), h0]),
+        (lambda x, r, w, b, s: S.add_norm(x, r, w, b, scale=s)[0], [rows(), rows(), per(), per(), per()]),
+        (lambda x, z, w, b: S.gate_norm(x, z, w, b), [rows(), rows(), per(), per()]),
+    ]
+    for f, ins in calls:
+        dy = rows()
+        leaves = [t.clone().requires_grad_() for t in ins]
+        want = torch.autograd.grad(f(*leaves), leaves, dy)
+        for free in range(len(ins)):
+            leaves = [t.clone().requires_grad_(i == free) for i, t in enumerate(ins)]
+            f(*leaves).backward(dy)
+            for i, t in enumerate(leaves):
+                assert (t.grad is None) == (i != free)
+            assert torch.equal(leaves[free].grad, want[free])
+
+
 # ---- float32 results of 16-bit rows ---------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", TYPES)
 def test_float32_results_carry_float32_functions(gpu, dtype):
@@ -202,6 +230,45 @@ def test_tokens_give_the_bits_of_the_prompt(gpu, dtype):
     state = torch.zeros(1, 3, ch, dtype=dtype, device=gpu)
     tokens = S.causal_conv_step(x, state, w, b, activation="silu", slots=torch.zeros(rows, dtype=torch.int32, device=gpu))
     assert torch.equal(tokens, whole) and torch.equal(state, last)
+
+
+# ---- the scan's gradients, element by element -------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", range(len(SCAN)))
+def test_selective_scan_gradients(gpu, case, dtype):
+    """Every gradient with initial states and a gradient of the final ones, against bounds from each element's own
+    terms (tests/test_sequence_cpu.py shows that a gradient of zero, or one without its A or its B term, breaks them)."""
+    import speech_to_text_amd as S
+
+    args, init, dy, dstate, off, plus, clean = R.scan_gradient_case(gpu, SCAN[case], dtype, 300 + case, scan_case)
+    grads = S.selective_scan_backward(dy, *args, off, softplus=plus, initial_state=init, dstate=dstate)
+    refs, sizes, steps = R.scan_gradients(dy, *args, off.tolist(), plus, init, dstate, clean)
+    for k, ref in refs.items():
+        got = getattr(grads, k)
+        if k in ("u", "delta", "B", "C"):
+            assert (got[clean:] == 0).all(), k
+            got = got[:clean]
+        R.assert_close(got, ref, F32 if k in ("A", "D", "delta_bias", "initial_state") else dtype, sizes[k], steps[k], k)
+
+
+def test_scan_into_a_column_range(gpu):
+    """`out` with rows further apart than its channels: the rows of sequences are those of a plain call, the rest of
+    the matrix stays as it was."""
+    import speech_to_text_amd as S
+
+    g = gen(gpu, 61)
+    for dtype in TYPES:
+        for rows, ch, n in ((90, 33, 5), (20, 7, 3), (700, 130, 16)):
+            u, delta = randn(g, rows, ch, dtype=dtype), randn(g, rows, ch, dtype=dtype)
+            B, C, A = randn(g, rows, n, dtype=dtype), randn(g, rows, n, dtype=dtype), -rand(g, ch, n, lo=0.1)
+            off = [3, 9, 9, rows - 2]
+            want = S.selective_scan(u, delta, A, B, C, None, None, off, softplus=True)
+            base = torch.full((rows, ch + 11), 3.0, dtype=dtype, device=gpu)
+            out = base[:, 4:4 + ch]
+            assert S.selective_scan(u, delta, A, B, C, None, None, off, softplus=True, out=out) is out
+            assert torch.equal(out[3:rows - 2], want[3:rows - 2])
+            assert (out[:3] == 3).all() and (out[rows - 2:] == 3).all()
+            assert (base[:, :4] == 3).all() and (base[:, 4 + ch:] == 3).all()
 
 
 # ---- refusals -----------------------------------------------------------------------------------------------------------

@@ -229,3 +229,28 @@ def test_references_against_differences():
         assert check(lambda x, q, w, b, s: R.add_norm(x, q, w, b, s, kind), r(3, 5), r(3, 5), r(5), r(5), r(5))
         for first in (True, False):
             assert check(lambda x, z, w, b: R.gate_norm(x, z, w, b, kind, 2, first), r(3, 6), r(3, 6), r(6), r(6))
+
+
+@pytest.mark.parametrize("case", range(10))
+def test_bounds_of_the_scan_gradients(case):
+    """What the GPU test of every scan gradient allows is less than any of them, and than either part of delta's: its
+    way through B u and its way through the decays."""
+    from tests.test_gpu_sequence import SCAN, scan_case
+
+    for dtype in (torch.float32, torch.bfloat16):
+        args, init, dy, dstate, off, plus, clean = R.scan_gradient_case(torch.device("cpu"), SCAN[case], dtype, 300 + case, scan_case)
+        refs, sizes, steps = R.scan_gradients(dy, *args, off.tolist(), plus, init, dstate, clean)
+        u, delta, A, B, C, D, bias = R.leaves(*args, grad=False)
+        raw = (delta if bias is None else delta + bias)[:clean]
+        d, slope = (R.softplus(raw), torch.sigmoid(raw)) if plus else (raw, 1.0)
+        by_B = u[:clean] * (refs["u"] - (0 if D is None else D * dy[:clean].double())) / d * slope
+        parts = dict(refs, **{"delta without B": by_B, "delta without its decays": refs["delta"] - by_B})
+        for k, missing in parts.items():
+            name = k.split()[0]
+            kind = torch.float32 if name in ("A", "D", "delta_bias", "initial_state") else dtype
+            ref = refs[name]
+            assert (ref.abs() <= sizes[name] * (1 + 1e-9)).all(), k
+            got = refs["delta"] - missing if " " in k else torch.zeros_like(ref)
+            with pytest.raises(AssertionError, match="beyond the bound"):
+                R.assert_close(got, ref, kind, sizes[name], steps[name], name)
+            R.assert_close(ref, ref, kind, sizes[name], steps[name], name)
