@@ -1108,9 +1108,13 @@ int scan_step(const mfcc_scan_args* a, int n_slots, const int32_t* slots, hipStr
     return by_state(a->state, [&](auto np) {
         constexpr int NP = decltype(np)::value;
         const int64_t tiles = ceil_div((int64_t)a->channels * (NP / 4), 256);
-        // four entries per thread share A and one look through the list of slots: 2048 x 1024 60 -> 51 us, but
-        // 256 x 4096 28 -> 29 us and 8 x 512 3.2 -> 4.8 us
-        if (f.batch >= 512)
+        // Four entries per thread share A and one look through the list of slots, but are a quarter of the wavefronts.  By
+        // the wavefronts of one entry per thread (entries x channels x states), one and four, in us: 4096 (512 x 256 x 8) 4.3
+        // and 5.0; 16384 (1024 x 256 x 16) 9.6 and 9.1, without slots 7.9 and 8.0; 65536 (1024 x 1024 x 16) 29.3 and 28.7, without
+        // slots 24.2 and 25.7; 131072 (2048 x 1024 x 16) 60.5 and 51.3, without 45.5 and 44.9, few entries (128 x 4096 x 64)
+        // 54.6 and 50.2; 65536 of few entries (256 x 4096 x 16) 29.0 and 29.4.
+        const int64_t waves = ceil_div((int64_t)a->channels * (NP / 4), WAVE) * f.batch;
+        if (waves >= 96 * 1024 || (slots && f.batch >= 512 && waves >= 12 * 1024))
             hipLaunchKernelGGL((k_scan_step<T, NP, 4>), dim3((unsigned)tiles, (unsigned)ceil_div(f.batch, 4)), dim3(256), 0, st, f);
         else
             hipLaunchKernelGGL((k_scan_step<T, NP, 1>), dim3((unsigned)tiles, (unsigned)f.batch), dim3(256), 0, st, f);

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from tests import sequence_ref as R
-from tests.test_gpu_sequence import F32, SCAN, TYPES, device_offsets, gen, rand, randn, scan_case
+from tests.test_gpu_sequence import BF16, F32, SCAN, TYPES, device_offsets, gen, rand, randn, scan_case
 
 pytestmark = pytest.mark.gpu
 
@@ -269,6 +269,38 @@ def test_scan_into_a_column_range(gpu):
             assert torch.equal(out[3:rows - 2], want[3:rows - 2])
             assert (out[:3] == 3).all() and (out[rows - 2:] == 3).all()
             assert (base[:, :4] == 3).all() and (base[:, 4 + ch:] == 3).all()
+
+
+# ---- single tokens: one and four entries per thread ------------------------------------------------------------------
+@pytest.mark.parametrize("batch,ch,n,listed", [(603, 400, 16, True), (603, 400, 16, False), (511, 400, 16, True), (527, 30, 8, True),
+                                               (131, 3001, 64, True), (131, 3001, 64, False)])
+def test_scan_step_by_wavefronts(gpu, batch, ch, n, listed):
+    """Around the sizes where a thread takes four entries: each as a call of its own, slots out of order and one twice."""
+    import speech_to_text_amd as S
+
+    g = gen(gpu, batch + ch)
+    u, delta = randn(g, batch, ch, dtype=BF16), randn(g, batch, ch, dtype=BF16)
+    B, C, A, D = randn(g, batch, n, dtype=BF16), randn(g, batch, n, dtype=BF16), -rand(g, ch, n, lo=0.1, hi=2.0), randn(g, ch)
+    pool = randn(g, batch, ch, n)
+    slots = None
+    if listed:
+        slots = torch.randperm(batch, generator=g, device=gpu).to(torch.int32)
+        slots[7], slots[batch - 1] = -1, slots[5]
+    got = pool.clone()
+    y = S.selective_scan_step(u, delta, A, B, C, got, D, softplus=True, slots=slots)
+    few = list(range(0, batch, max(1, batch // 20))) + [5, 7, batch - 2, batch - 1]
+    for i in sorted(set(few)):
+        at = i if slots is None else int(slots[i])
+        if at < 0:
+            assert (y[i] == 0).all()
+            continue
+        one = pool[at:at + 1].clone()
+        if listed and i == batch - 1:                       # the second token of its sequence
+            S.selective_scan_step(u[5:6], delta[5:6], A, B[5:6], C[5:6], one, D, softplus=True)
+        want = S.selective_scan_step(u[i:i + 1], delta[i:i + 1], A, B[i:i + 1], C[i:i + 1], one, D, softplus=True)
+        assert torch.equal(y[i], want[0])
+        if not (listed and i == 5):
+            assert torch.equal(got[at], one[0])
 
 
 # ---- refusals -----------------------------------------------------------------------------------------------------------
