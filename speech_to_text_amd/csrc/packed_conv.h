@@ -40,11 +40,10 @@ __device__ __forceinline__ void load_taps(float (&w)[K][VEC], float (&b)[VEC], c
     }
 }
 
-// p, or p sigmoid(p), of the forward pass and of single tokens: one function, so that tokens give the prompt's bits.  In
-// 16-bit types y is all there is of it (30011 x 4096: 97 us, 101 us with sigmoid_f).
+// p sigmoid(p) of the forward pass and of single tokens: one function, so that tokens give the prompt's bits.  In 16-bit
+// types y is all there is of it (30011 x 4096: 98 us, 101 us with sigmoid_f).
 template <typename M>
-__device__ __forceinline__ float activated(int act, float p) {
-    if (!act) return p;
+__device__ __forceinline__ float silu_f(float p) {
     return p * (sizeof(M) == 4 ? sigmoid_f(p) : sigmoid_to_16(p));
 }
 
@@ -94,8 +93,10 @@ __global__ __launch_bounds__(256) void k_conv_fwd(const ConvFwd a) {
     load_taps<K, VEC>(w, b, a.w, a.bias, c0, n);
     Place q = find_row(a.off, a.n_seqs, a.rows, r0);
     auto finish = [&](float (&acc)[VEC], int64_t row) {
+        if (a.act) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) acc[i] = activated<M>(a.act, acc[i]);
+            for (int i = 0; i < VEC; ++i) acc[i] = silu_f<M>(acc[i]);
+        }
         store_vec<M, VEC>(y + row * a.y_stride, acc, n);
     };
     for (int64_t r = r0; r < r1; r += G) {
@@ -455,7 +456,7 @@ __global__ __launch_bounds__(256) void k_conv_step(const ConvStep a) {
             acc[i] = b[i];
 #pragma unroll
             for (int j = 0; j < K; ++j) acc[i] = fmaf(w[j][i], win[j][i], acc[i]);
-            acc[i] = activated<M>(a.act, acc[i]);
+            if (a.act) acc[i] = silu_f<M>(acc[i]);
         }
         store_vec<M, VEC>(y + (int64_t)e * a.y_stride, acc, n);
 #pragma unroll

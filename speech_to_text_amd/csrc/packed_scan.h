@@ -26,11 +26,8 @@ constexpr int ZERO_ROW = SCAN_TILE;  // behind them one of zeros, for the missin
 // A log2(e), so that a decay is exp2(d rate): d A is rounded twice where exp(d A) would round it once, and a decay over
 // rows with sum |d A| = X is off by up to X 2^-23 of itself.  For A <= 0 that is at most 2^-23 / e of the state (X exp(-X)
 // <= 1 / e).  A second float of the product would cost two more operations per element, of five.  Also, a step of
-// zero (a missing row too) decays by one whatever the rate: a product beyond the range of float32 becomes the largest number.
-__device__ __forceinline__ float rate_of(float A) {
-    const float r = A * LOG2E;
-    return fabsf(r) > 3.40282347e38f ? copysignf(3.40282347e38f, r) : r;
-}
+// zero (a missing row too) decays by one whatever the rate: beyond the range of float32 it is the lowest number.
+__device__ __forceinline__ float rate_of(float A) { return __builtin_elementwise_maximum(A * LOG2E, -3.40282347e38f); }   // a NaN stays
 
 // Holds the LDS reads of the next row back until half of this row's states are done: hoisted by the compiler,
 // the B and C of four rows take the registers of two wavefronts.
@@ -284,7 +281,6 @@ __global__ __launch_bounds__(256) void k_scan_sum(const Scan a) {
 template <typename T, int BATCH>
 __global__ __launch_bounds__(1024) void k_scan_carry(const Scan a) {
     __shared__ float sD[16][64], sH[16][64];
-    __shared__ int s_cut[16];
     const int lane = threadIdx.x & 63, seg = threadIdx.x >> 6;
     const bool right = blockIdx.y == 1;
     float* st = right ? a.gst : a.hst;
@@ -309,23 +305,20 @@ __global__ __launch_bounds__(1024) void k_scan_carry(const Scan a) {
         for (int j = 0; j < BATCH; ++j) dec[j] = exp2_hw(A2 * dec[j]);
     };
     float D = 1.0f, H = 0.0f;
-    int any_cut = 0;
     for (int i0 = k0; i0 < k1; i0 += BATCH) {
         fetch(i0);
 #pragma unroll
         for (int j = 0; j < BATCH; ++j)
             if (i0 + j < k1) {
                 H = cut[j] ? v[j] : fmaf(dec[j], H, v[j]);
-                D *= dec[j];
-                any_cut |= cut[j];
+                D = cut[j] ? -1.0f : D * dec[j];           // the sign, which no decay changes, says that there was a cut
             }
     }
     sD[seg][lane] = D; sH[seg][lane] = H;
-    if (lane == 0) s_cut[seg] = any_cut;                   // the same for all columns
     __syncthreads();
     float carry = 0.0f;
     // what comes before a cut does not pass it; what comes before decays whose product is zero does, if it is a NaN
-    for (int s = 0; s < seg; ++s) carry = s_cut[s] ? sH[s][lane] : fmaf(sD[s][lane], carry, sH[s][lane]);
+    for (int s = 0; s < seg; ++s) carry = signbit(sD[s][lane]) ? sH[s][lane] : fmaf(sD[s][lane], carry, sH[s][lane]);
     for (int i0 = k0; i0 < k1; i0 += BATCH) {
         if (len > BATCH) fetch(i0);                    // a shorter segment is still in registers
 #pragma unroll
