@@ -73,7 +73,7 @@ struct Raw {
 // element by element.
 // Elements behind a row's last are read along with it where the tensor goes on behind the row (any row but the last,
 // rows at least VEC - 1 apart) and thrown away: taking the last n < VEC one by one in a 16-bit type packs them where they
-// are loaded, and so waits for every load in flight (gradients of the gated norm at 12001 x 1545 88 instead of 58 us).
+// are loaded, and so waits for every load in flight (gradients of the gated norm at 12001 x 1545 in bfloat16 54 instead of 48 us).
 inline bool has_room(const void* p, int64_t stride, int vec) { return !p || stride >= vec - 1; }
 
 template <typename M, int VEC>

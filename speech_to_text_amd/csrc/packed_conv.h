@@ -188,7 +188,7 @@ struct ConvBwd {
 // dp = dy * act'(p) is formed for the tile's rows and the K - 1 rows behind it; dx[o] gathers the K values
 // of dp that read row o, and the products dp * x add up to the tile's share of dweight.
 // Three rows of traffic and 2 K registers of sums per channel: fewer wavefronts than the forward pass has.  30011 x
-// 4096, K = 4: 191 us in bfloat16 (3.9 TB/s), 326 us in float32 (4.5 TB/s); 6001 x 1545, K = 3, float32: 36 us.
+// 4096, K = 4: 187 us in bfloat16 (3.9 TB/s), 326 us in float32 (4.5 TB/s); 6001 x 1545, K = 3, float32: 36 us.
 template <typename T, int K, int VEC>
 __global__ __launch_bounds__(256) void k_conv_bwd(const ConvBwd a) {
     using M = typename T::mem;
@@ -475,7 +475,7 @@ constexpr int CONV_AHEAD = 8;      // rows in flight of the forward pass
 
 // Rows per thread of the forward pass: a long tile reads its taps and the K - 1 rows of overlap less often, but
 // below about eight wavefronts per SIMD (256 CUs x 4) the chip is not full.  16 rows throughout, 128 throughout, and
-// so, K = 4, bfloat16: 600 x 512 7.5, 30 and 6.0 us; 30011 x 4096 85, 94 and 86 us.
+// so, K = 4, bfloat16: 600 x 512 7.8, 31 and 6.2 us; 4000 x 1024 9.2, 33 and 7.3 us; 30011 x 4096 100, 103 and 98 us.
 inline int conv_fwd_tile(int64_t rows, int n_vec) {
     for (int tile : {128, 64, 32, 16})
         if (ceil_div(rows, tile) * n_vec >= 8 * 1024 * WAVE) return tile;
@@ -483,8 +483,9 @@ inline int conv_fwd_tile(int64_t rows, int n_vec) {
 }
 
 // Rows per wavefront of the backward pass (it also reads K - 1 rows of overlap and writes K + 1 partial sums per four
-// tiles).  K = 4, bfloat16, with the summing launch, by tiles of 4, 8, 16 and 128 rows: 600 x 512 11.7, 15, 20, 86 us;
-// 4000 x 1024 20.1, 19.4, 22, 88; 12000 x 1024 38, 32, 29, -; 30011 x 4096 -, -, 185, 183.
+// tiles).  K = 4, bfloat16, with the summing launch, by tiles of 4, 8, 16 and 128 rows: 600 x 512 11, 13, 18, 88 us; 4000
+// x 1024 21, 18, 20, 89; 12000 x 1024 40, 33, 28, 90.  By 16, 32, 64 and 128 rows: 30011 x 2048 102, 94, 94, 112 us; 30011 x
+// 4096 201, 179, 187, 172; 20000 x 8192 257, 238, 232, 239: within 9 % of the best tile.
 inline int conv_bwd_tile(int64_t rows, int n_vec) {
     const int64_t across = ceil_div(n_vec, WAVE);
     for (int tile : {128, 64, 32})

@@ -4,8 +4,8 @@
 //   norm:  v / sqrt(mean(v^2) + eps), of v - mean(v) for the layer form.
 // Bound by memory: every row is read once, held in registers (eight neighbouring elements a thread and
 // step), reduced over 16 to 1024 threads and written once.  The layer form's deviation is summed
-// around the mean, from the registers.  16384 x 2048, bfloat16 with a float32 residual: 82 us forward (4.9 TB/s), 120 us
-// backward (5.0 TB/s); the gate over 30011 x 4096 in 8 groups, bfloat16: 134 us (5.5 TB/s).
+// around the mean, from the registers.  16384 x 2048, bfloat16 with a float32 residual: 82 us forward (4.9 TB/s), 118 us
+// backward (5.1 TB/s); the gate over 30011 x 4096 in 8 groups, bfloat16: 136 us (5.4 TB/s, two reads to a write).
 #pragma once
 #include "packed.h"
 
@@ -324,7 +324,8 @@ void k_norm_bwd(const Norm a) {
 // A row wider than the registers of a workgroup hold is read twice (three times for the layer form, whose deviation
 // is summed around the mean), the second time from a cache.  The sums over rows are left to k_norm_columns, which
 // reads everything once more with a thread per eight columns and takes the row's statistics from the workspace.
-// Bound by memory: 1000 x 32768 in 122 us in bfloat16, 250 us in float32 (2.1 TB/s of the four tensors, each read twice).
+// Bound by memory: 1000 x 32768 in 104 us in bfloat16 and 237 us in float32 (2.5 and 2.2 TB/s of the residual norm's four
+// tensors, those that are read twice counted once); the gate 130 and 288 us.
 
 // Eight columns of a row.
 template <typename T, typename RT, bool GATE>
@@ -480,8 +481,8 @@ __global__ __launch_bounds__(1024) void k_norm_reduce(const float* __restrict__ 
 constexpr int NORM_MAX_WIDTH = 32768;
 
 // Threads per row and steps of eight elements per thread: (16, 1) .. (1024, 4).  As few threads as hold the row in one
-// step: their sums need fewer exchanges and no lanes idle (gradients of 30011 x 1000 in bfloat16 57 us with 128
-// threads, 91 us with 256).
+// step: their sums need fewer exchanges and no lanes idle (gradients of 30011 x 1000 in bfloat16 42 us with 128
+// threads, 61 us with 256; of the gate 58 and 95 us).
 template <int MOST, typename Fn>
 int by_width_of_row(int width, Fn&& fn) {
     using std::integral_constant;
@@ -498,8 +499,8 @@ int by_width_of_row(int width, Fn&& fn) {
     }
 }
 
-// Rows up to this width stay in registers in the gradients too (4000 x 8192 bfloat16: 72 us, against 130 us by
-// k_norm_bwd_wide); wider ones would spill (1000 x 20000: 368 us, against 83 us).
+// Rows up to this width stay in registers in the gradients too (4000 x 8192 bfloat16: 60 us, the gate 82 us, against 107 and
+// 146 us by k_norm_bwd_wide); wider ones would spill (the gate at 1000 x 20000: 368 us, against 88 us).
 constexpr int NORM_HELD = 8192;
 
 // Blocks that walk over the rows in the backward pass, each with a row of partial sums: about four wavefronts for

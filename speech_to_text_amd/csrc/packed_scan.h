@@ -9,11 +9,13 @@
 // local part needs the running product of the a_t only, so pass 1 forms both with one exp per element.
 // A chunk that holds the start of a sequence lets nothing through (its decay counts as zero).
 //
-// Bound by vector issue, not memory: per (row, channel, n) one exp (8 SIMD cycles per wavefront) and four to
-// five plain operations (2.6 each) per pass against 6 / N bytes in 16-bit types.  16384 x 2048, 16 states, bfloat16:
-// 116 + 10 + 147 us for the three passes (the two sweeps 4.6 and 3.7 10^12 elements (row, channel, n) a second).
-// In both 80 % of the issue slots are taken.  The first sweep is what the split costs; undivided, 2048 channels are
-// 32 wavefronts for 1024 SIMDs.
+// Bound by vector issue, not memory: per (row, channel, n) and pass one exp and four to five plain operations, against
+// 6 / N bytes in 16-bit types.  A SIMD has one issue slot in four cycles.  An exp takes two; a plain operation takes one, or
+// half where it is issued in a pair with one of another wavefront (2.6 cycles in a loop of nothing else).  16384 x 2048,
+// 16 states, bfloat16: 118 + 11 + 150 us for the three passes.  By the counters the first sweep issues 50 M instructions (9.5 M
+// of them exp and log), a third of them in pairs, in 51 M slots: 82 % of the slots of busy CUs, and CUs are busy 90 % of
+// the time.  The last one issues 63 M, 36 % in pairs, in 61 M slots, 78 %.  With pairs throughout both would take two thirds of
+// their time.  The first sweep is what the split costs; undivided, 2048 channels are 32 wavefronts for 1024 SIMDs.
 #pragma once
 #include "packed.h"
 
@@ -277,7 +279,7 @@ __global__ __launch_bounds__(256) void k_scan_sum(const Scan a) {
 // Pass 2, in place: hst[k] (and, from the right, gst[k]) becomes the state that enters chunk k.  64 columns
 // by 16 segments of the chunks: each segment's own composition, then the ones before it, then the segment.
 // BATCH chunks are loaded at a time: one after the other they are a chain of memory latencies.  Bound by memory:
-// 128 chunks of 2048 x 16 states read and written in 10 us (3.3 TB/s).
+// 128 chunks of 2048 x 16 states read and written in 11 us (3.1 TB/s).
 template <typename T, int BATCH>
 __global__ __launch_bounds__(1024) void k_scan_carry(const Scan a) {
     __shared__ float sD[16][64], sH[16][64];
@@ -332,7 +334,7 @@ __global__ __launch_bounds__(1024) void k_scan_carry(const Scan a) {
 }
 
 // Pass 3: y, and the states that sequences leave behind.  A lane holds a channel with all its states, so that the sum
-// over them needs no other lane.  Four rows of u and delta are in flight; 147 us at 16384 x 2048 x 16 in bfloat16.
+// over them needs no other lane.  Four rows of u and delta are in flight; 150 us at 16384 x 2048 x 16 in bfloat16.
 template <typename T, int NP>
 __global__ __launch_bounds__(256) void k_scan_fwd(const Scan a) {
     using M = typename T::mem;
@@ -455,8 +457,8 @@ __global__ __launch_bounds__(1024) void k_scan_empty(const Empties a) {
 // latencies overlap.  Sums over n stay in the LPC lanes of a channel; dB and dC are summed over the channels of the
 // wavefront (v_permlane swaps halve eight values to two, then rotations within a row of lanes), over the four
 // wavefronts in LDS, and over the workgroups of a group by k_scan_reduce: a fixed order throughout.
-// Bound by vector issue: 113 instructions per wavefront and row (256 elements), eight of them an exp; 80 % of
-// the issue slots are taken (an exp takes two).  12007 x 2048 x 16 in bfloat16: 415 us.
+// Bound by vector issue: 118 instructions per wavefront and row (256 elements), eight of them an exp, 29 % of them issued in
+// pairs: 109 slots, 76 % of those of busy CUs (an exp takes two).  12007 x 2048 x 16 in bfloat16: 405-417 us.
 constexpr int SUB = 8;
 
 template <int NP> constexpr int bwd_lpc() { return NP / 4; }
@@ -925,7 +927,7 @@ inline int sum_slices(int state, bool back) { return (int)ceil_div(state, sum_st
 // long ones are preferred while they leave about four wavefronts for every SIMD (256 CUs x 4).  Smaller problems
 // are bound by the time of one wavefront, which goes with its rows (0.6 us each), and take shorter chunks; up to
 // 32 rows one pass is faster than three launches.  With 16 rows throughout, 128 throughout, and so: 1187 x 518 x 16
-// 31, 107 and 31 us, 12007 x 2048 x 16 350, 238 and 234 us.
+// 28, 103 and 28 us, 12007 x 2048 x 16 248, 197 and 193 us, 300 x 256 x 16, where so is 8, 25, 103 and 20 us.
 inline int scan_fwd_chunk(const mfcc_scan_args* a) {
     if (a->rows <= 32) return 32;
     const int64_t waves = (int64_t)a->groups * ceil_div(a->channels / a->groups, WAVE);
@@ -936,7 +938,7 @@ inline int scan_fwd_chunk(const mfcc_scan_args* a) {
 }
 
 // Rows per chunk of the gradients, by the same trade.  16 rows throughout, as many as fit, and so: 1187 x 518 x 16
-// 43, 73 and 44 us; 12007 x 2048 x 16 761, 595 and 595 us; 300 x 256 x 16, where so is 8: 31, 64 and 29 us.
+// 43, 66 and 43 us; 12007 x 2048 x 16 680, 534 and 534 us; 300 x 256 x 16, where so is 8: 29, 62 and 27 us.
 inline int bwd_channels_of(int np) { return 4 * WAVE / (np / 4); }
 inline int scan_bwd_chunk(const mfcc_scan_args* a) {
     const int cpb = bwd_channels_of(padded_state(a->state)), most = cpb >= 256 ? 16 : cpb >= 128 ? 32 : 64;
@@ -1009,7 +1011,7 @@ inline int64_t carry_blocks(const Scan& f) { return ceil_div((int64_t)f.state * 
 template <typename T>
 void launch_carry(const Scan& f, unsigned directions, hipStream_t st) {
     const dim3 grid((unsigned)carry_blocks(f), directions);
-    // 1187 x 518 x 16 (75 chunks) 7 and 11 us; 2500 x 700 (157) 16 and 13, 12007 x 2048 (188) 32 and 28 us
+    // 1187 x 518 x 16 (75 chunks) 7 and 11 us; 2500 x 700 (157) 16 and 13, 12007 x 2048 (188) 34 and 29 us
     if (f.n_chunks <= 16 * 8) hipLaunchKernelGGL((k_scan_carry<T, 8>), grid, dim3(1024), 0, st, f);
     else hipLaunchKernelGGL((k_scan_carry<T, 16>), grid, dim3(1024), 0, st, f);
 }
