@@ -131,14 +131,14 @@ __device__ __forceinline__ float sigmoid_f(float x) { return rcp_hw(1.0f + exp_f
 
 // For a result that is rounded to 16 bits and goes nowhere else: without the second float of the exponent's product
 // the sigmoid is off by |x| 2^-24 more, below 2^-17 up to |x| = 88, where it leaves float32's range; half a step of
-// bfloat16 is 2^-9 of the value, of float16 2^-12.  Whatever has float32 results takes sigmoid_f.
+// bfloat16 is up to 2^-8 of the value, of float16 2^-11.  Whatever has float32 results takes sigmoid_f.
 __device__ __forceinline__ float sigmoid_to_16(float x) { return rcp_hw(1.0f + exp2_hw(x * -LOG2E)); }
 
 // log(1 + exp(x)) = max(x, 0) + log(1 + e), e = exp(-|x|) in (0, 1].  w = 1 + e loses the low bits of a
 // small e; what it lost, e - (w - 1), is exact and is added back (to first order: the error of that is
 // below 2^-24 e).
 __device__ __forceinline__ float softplus_f(float x) {
-    // exp_f of -|x|, which -100 does not change (its exp is below the smallest float32) but for the infinity it takes away
+    // exp_f of -|x|: the bound takes away the infinity and changes nothing else (exp(-100) is below float32's normal range)
     const float v = __builtin_elementwise_maximum(-fabsf(x), -100.0f);     // a NaN stays
     const float p = v * LOG2E, e0 = exp2_hw(p), e = fmaf(e0, exp_rest(v, p), e0);
     const float w = 1.0f + e;

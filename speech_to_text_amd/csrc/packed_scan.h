@@ -9,13 +9,14 @@
 // local part needs the running product of the a_t only, so pass 1 forms both with one exp per element.
 // A chunk that holds the start of a sequence lets nothing through (its decay counts as zero).
 //
-// Bound by vector issue, not memory: per (row, channel, n) and pass one exp and four to five plain operations, against
-// 6 / N bytes in 16-bit types.  A SIMD has one issue slot in four cycles.  An exp takes two; a plain operation takes one, or
-// half where it is issued in a pair with one of another wavefront (2.6 cycles in a loop of nothing else).  16384 x 2048,
-// 16 states, bfloat16: 118 + 11 + 150 us for the three passes.  By the counters the first sweep issues 50 M instructions (9.5 M
-// of them exp and log), a third of them in pairs, in 51 M slots: 82 % of the slots of busy CUs, and CUs are busy 90 % of
-// the time.  The last one issues 63 M, 36 % in pairs, in 61 M slots, 78 %.  With pairs throughout both would take two thirds of
-// their time.  The first sweep is what the split costs; undivided, 2048 channels are 32 wavefronts for 1024 SIMDs.
+// Bound by vector issue, not memory: per (row, channel, n) one exp and three plain operations in the first sweep, four in
+// the last one, against 6 / N bytes in 16-bit types.  A SIMD has one issue slot in four cycles.  An exp takes two; a plain
+// operation takes one, or half where it is issued in a pair with one of another wavefront (2.6 cycles in a loop of
+// nothing else).  16384 x 2048, 16 states, bfloat16: 118 + 11 + 150 us for the three passes.  By the counters the first
+// sweep issues 50 M instructions (9.5 M of them exp and log), a third of them in pairs, in 51 M slots: 81 % of the slots of
+// busy CUs, and CUs are busy 90 % of the time.  The last one issues 63 M, 36 % in pairs, in 61 M slots, 78 %.  With pairs
+// throughout both would take two thirds of their time; a third of the instructions is softplus, staging and the loop.
+// The first sweep is what the split costs: undivided, 2048 channels are 32 wavefronts for 1024 SIMDs.
 #pragma once
 #include "packed.h"
 
@@ -27,7 +28,7 @@ constexpr int ZERO_ROW = SCAN_TILE;  // behind them one of zeros, for the missin
 
 // A log2(e), so that a decay is exp2(d rate): d A is rounded twice where exp(d A) would round it once, and a decay over
 // rows with sum |d A| = X is off by up to X 2^-23 of itself.  For A <= 0 that is at most 2^-23 / e of the state (X exp(-X)
-// <= 1 / e).  A second float of the product would cost two more operations per element, of five.  Also, a step of
+// <= 1 / e).  A second float of the product would cost two more operations per element, to four or five.  Also, a step of
 // zero (a missing row too) decays by one whatever the rate: beyond the range of float32 it is the lowest number.
 __device__ __forceinline__ float rate_of(float A) { return __builtin_elementwise_maximum(A * LOG2E, -3.40282347e38f); }   // a NaN stays
 
